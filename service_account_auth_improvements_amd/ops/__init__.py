@@ -282,6 +282,96 @@ def cross_entropy_grad_(logits, labels, lse, scale, vocab_start, ignore_index=-1
     return logits
 
 
+# ---------------------------------------------------------------- token log-probabilities
+def token_logprobs_fwd(logits, tokens, temperature=1.0, top=0, ignore_index=-100):
+    """Log-probabilities of given tokens, with each row's entropy and its top alternatives.
+
+    logits [T, V] bf16 / fp16 / fp32 with unit inner stride (any row stride); tokens int64 [T].
+    ``temperature`` (1e-4 to 1e4) divides the logits.  Returns ``(logp [T], entropy [T], stats [T, 2],
+    top_ids [T, top] int64, top_logp [T, top])``, fp32 in nats; ``stats`` is what
+    :func:`token_logprobs_bwd` needs.  ``top`` (at most 128 and V) alternatives are ordered by
+    descending logit, equal logits by ascending id, NaN first.  Rows whose token is
+    ``ignore_index`` are padding: they are not read, give 0 and ids of -1.  A token outside the
+    vocabulary gives NaN; a row with NaN, with +inf or with nothing but -inf is NaN.  The whole
+    vocabulary is expected in one row: under tensor parallelism gather the shards' logits first."""
+    if logits.is_cuda:
+        return _k().token_logprobs(logits, tokens, temperature, top, ignore_index)
+    return reference.token_logprobs(logits, tokens, temperature, top, ignore_index)
+
+
+def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp=None, dentropy=None, temperature=1.0,
+                       ignore_index=-100, out=None):
+    """Gradient of :func:`token_logprobs_fwd`'s logp and entropy: dlogits in the logits' type, for
+    upstream gradients ``dlogp`` / ``dentropy`` (fp32 [T], None: zero).  ``out``: where to write it;
+    ``out=logits`` overwrites them."""
+    if out is None:
+        out = logits.new_empty(logits.shape)
+    if logits.is_cuda:
+        _k().token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperature, ignore_index, out)
+        return out
+    return reference.token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperature, ignore_index, out)
+
+
+# ---------------------------------------------------------------- distillation from top logits
+DISTILL_FUSED, DISTILL_STATS, DISTILL_GRAD = 0, 1, 2
+
+
+def _distill(logits, ids, z, lse, temperature, scale, rows, vocab_start, vocab_size, mode, stats, out):
+    if mode != DISTILL_STATS and out is None:
+        out = logits.new_empty(logits.shape)
+    fn = _k().distill_topk if logits.is_cuda else reference.distill_topk
+    st, sh = (scale, 0.0) if torch.is_tensor(scale) else (None, float(scale))
+    loss, part = fn(logits, ids, z, lse, temperature, st, sh, rows, vocab_start,
+                    logits.shape[1] if vocab_size is None else vocab_size, mode, stats, out)
+    return loss, part if mode == DISTILL_STATS else out
+
+
+def distill_topk_fused(logits, teacher_ids, teacher_logits, scale, temperature=1.0, teacher_lse=None, out=None):
+    """Distillation from a teacher's top logits, loss and gradient in one launch.
+
+    Per row, with p the softmax of ``logits`` [T, V] (bf16 / fp16 / fp32) at ``temperature``:
+    the divergence of p from the teacher's distribution q over the row's K entries,
+    ``sum q (ln q - ln p_id)``.  teacher_ids [T, K] int64 or int32 (negative: no entry; K <= 256),
+    teacher_logits [T, K] of any of the three types.  Without ``teacher_lse``, q is the softmax of the
+    entries.  With it (fp32 [T]: the log-sum-exp of the teacher's whole row at ``temperature``),
+    q = exp(z / temperature - lse), and the teacher's remaining mass is held against the student's
+    mass outside the ids as one bucket; V is at most 491520 then.  Log-probabilities serve as
+    teacher_logits (with a zero ``teacher_lse`` at temperature 1).
+
+    Returns (loss rows fp32 [T], dlogits).  dlogits are ``scale`` (a number or one fp32 on the
+    device) times the rows' gradients; ``out`` says where they go (``out=logits``: in place).
+    Neither is multiplied by temperature squared.  A row without entries gives 0; an id at or behind
+    the vocabulary's end gives NaN.  The same id may appear twice: its entries add up."""
+    return _distill(logits, teacher_ids, teacher_logits, teacher_lse, temperature, scale, None, 0, None, DISTILL_FUSED,
+                    None, out)
+
+
+def distill_topk_stats(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None, vocab_start=0,
+                       vocab_size=None):
+    """:func:`distill_topk_fused` of one vocabulary part (columns [vocab_start, vocab_start + V) of
+    ``vocab_size``; the teacher's ids are global), first half: this part's row statistics [T, 5].
+    Join the parts' with :func:`distill_topk_join`, then :func:`distill_topk_grad`."""
+    return _distill(logits, teacher_ids, teacher_logits, teacher_lse, temperature, 1.0, None, vocab_start, vocab_size,
+                    DISTILL_STATS, None, None)[1]
+
+
+def distill_topk_join(parts, temperature=1.0):
+    """Statistics [R, T, 5] of the R parts of a vocabulary -> the whole rows' [T, 4]."""
+    m, s, u, xq, q = parts.unbind(-1)
+    M = m.amax(0)
+    # a part (or row) of nothing but -inf: its sums are 0 whatever the shift
+    d = torch.where(torch.isneginf(m) | (m == M), torch.zeros_like(m), m - M)
+    f = torch.exp(d / temperature)
+    return torch.stack([M, (s * f).sum(0), (u * f).sum(0), (xq + torch.where(q == 0, q, q * d)).sum(0)], -1)
+
+
+def distill_topk_grad(logits, teacher_ids, teacher_logits, stats, scale, temperature=1.0, teacher_lse=None,
+                      vocab_start=0, vocab_size=None, out=None):
+    """Second half: (loss rows of the whole vocabulary, this part's dlogits) from joined ``stats``."""
+    return _distill(logits, teacher_ids, teacher_logits, teacher_lse, temperature, scale, None, vocab_start, vocab_size,
+                    DISTILL_GRAD, stats, out)
+
+
 # ---------------------------------------------------------------- AdamW (K6)
 def adamw_(p, w, m, v, g, n_decay, lr, b1, b2, eps, wd, step, gscale=1.0, sumsq=None,
            max_norm=0.0):
@@ -368,3 +458,66 @@ class _SwiGLUFn(torch.autograd.Function):
 
 def swiglu(gu):
     return _SwiGLUFn.apply(gu)
+
+
+def _refuse_live_leaf(x):
+    """A leaf's gradient accumulator belongs to the stream of the first graph that holds it.  A
+    backward pass captured on another stream while that graph lives would make the capture wait for
+    work outside it, which ends the process; the forward pass says so instead."""
+    if not (x.is_cuda and x.is_leaf and x.requires_grad and torch.is_grad_enabled()):
+        return
+    seen = torch.autograd.graph.get_gradient_edge(x).node.metadata
+    stream = torch.cuda.current_stream(x.device).cuda_stream
+    if seen.setdefault("kfamd_stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("these logits are a leaf of an earlier autograd graph that is still alive: drop that "
+                           "graph's outputs before capturing, or capture the _fwd / _bwd (or fused) calls")
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature, top, ignore_index):
+        logp, entropy, stats, ids, tlp = token_logprobs_fwd(logits, tokens, temperature, top, ignore_index)
+        ctx.save_for_backward(logits, tokens, stats, entropy)
+        ctx.args = temperature, ignore_index
+        ctx.mark_non_differentiable(ids, tlp)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, ids, tlp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogp, dent, _ids, _tlp):
+        if dlogp is None and dent is None:
+            return (None,) * 5
+        logits, tokens, stats, entropy = ctx.saved_tensors
+        c = lambda g: None if g is None else g.float().contiguous()   # noqa: E731
+        return (token_logprobs_bwd(logits, tokens, stats, entropy, c(dlogp), c(dent), *ctx.args),) + (None,) * 4
+
+
+def token_logprobs(logits, tokens, temperature=1.0, top=0, ignore_index=-100):
+    """:func:`token_logprobs_fwd` for autograd: (logp, entropy, top_ids, top_logp); the gradient runs
+    through logp and entropy."""
+    _refuse_live_leaf(logits)
+    return _TokenLogprobsFn.apply(logits, tokens, temperature, top, ignore_index)
+
+
+class _DistillTopkFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, z, temperature, lse):
+        loss, stats = _distill(logits, ids, z, lse, temperature, 1.0, None, 0, None, DISTILL_STATS, None, None)
+        ctx.save_for_backward(logits, ids, z, stats, *(() if lse is None else (lse,)))
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, drows):
+        logits, ids, z, stats, *lse = ctx.saved_tensors
+        _, d = _distill(logits, ids, z, lse[0] if lse else None, ctx.temperature, 1.0, drows.float().contiguous(), 0, None,
+                        DISTILL_GRAD, stats, None)
+        return d, None, None, None, None
+
+
+def distill_topk(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None):
+    """:func:`distill_topk_fused`'s loss rows for autograd (the teacher gets no gradient)."""
+    _refuse_live_leaf(logits)
+    return _DistillTopkFn.apply(logits, teacher_ids, teacher_logits, temperature, teacher_lse)

@@ -68,6 +68,15 @@ int kf_gemm_tn(const void*, long, const void*, long, void*, long, int, int, int,
 int kf_gemm_tn2(const void*, long, const void*, long, void*, long, int, int, const void*, long, const void*, long, void*,
                 long, int, int, int, int, hipStream_t);
 int kf_transpose_bf16(const void*, long, void*, long, int, int, hipStream_t);
+int kf_token_logprobs_top_max();
+int kf_token_logprobs(const void*, int, long, long, int, const long*, long, float, float*, float*, float*, int, long*,
+                      float*, hipStream_t);
+int kf_token_logprobs_bwd(const void*, int, long, void*, long, long, int, const long*, long, const float*, const float*,
+                          const float*, const float*, float, hipStream_t);
+int kf_distill_k_max();
+long kf_distill_rest_v_max();
+int kf_distill_topk(const void*, int, long, void*, long, long, int, long, long, const void*, int, long, const void*, int,
+                    long, const float*, int, float, const float*, float, const float*, float*, float*, long, int, hipStream_t);
 long kf_car_header_bytes();
 int kf_car_alloc(long, void**, void*);
 int kf_car_open(const void*, void**);
@@ -277,6 +286,158 @@ void cross_entropy_(at::Tensor logits, const at::Tensor& labels, int64_t vocab_s
                             labels.data_ptr<int64_t>(), vocab_start, ignore_index, loss.data_ptr<float>(),
                             lse.data_ptr<float>(), pm, ps, pxy, scp, (float)scale_h, (int)mode, cur_stream()),
            "cross_entropy");
+}
+
+// ---------------- token log-probabilities, distillation from top logits ----------------
+int float_type(const at::Tensor& t, const char* op, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
+    default: TORCH_CHECK(false, op, ": ", name, " must be bfloat16, float16 or float32"); return -1;
+  }
+}
+int check_logits(const at::Tensor& x, const char* op) {
+  TORCH_CHECK(x.is_cuda(), op, ": logits must be a GPU tensor");
+  const int dt = float_type(x, op, "logits");
+  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1 && x.size(1) < (1L << 31) - 64 && (x.size(1) == 1 || x.stride(1) == 1), op,
+              ": logits must be [T, V] with V >= 1 and unit inner stride");
+  return dt;
+}
+void check_temperature(double t, const char* op) {
+  TORCH_CHECK(t >= 1e-4 && t <= 1e4, op, ": temperature must be between 1e-4 and 1e4");
+}
+// fp32 [T, n] (n = 0: [T]) on x's device, contiguous
+void check_rows_f32(const at::Tensor& t, const at::Tensor& x, int64_t n, const char* op, const char* name) {
+  TORCH_CHECK(t.device() == x.device() && t.scalar_type() == at::kFloat && t.is_contiguous() &&
+                  t.dim() == (n ? 2 : 1) && t.size(0) == x.size(0) && (!n || t.size(1) == n),
+              op, ": ", name, " must be contiguous float32 [T", n ? ", " + std::to_string(n) : std::string(),
+              "] on the logits' device");
+}
+at::Tensor check_tokens(const at::Tensor& tok, const at::Tensor& x, const char* op) {
+  TORCH_CHECK(tok.device() == x.device() && tok.scalar_type() == at::kLong && tok.dim() == 1 && tok.size(0) == x.size(0),
+              op, ": tokens must be int64 [T] on the logits' device");
+  return tok.contiguous();
+}
+// where the gradient goes: the logits themselves, or a tensor that does not overlap them
+void check_grad_out(const at::Tensor& x, const at::Tensor& o, const char* op) {
+  const int64_t T = x.size(0), V = x.size(1);
+  TORCH_CHECK(o.device() == x.device() && o.scalar_type() == x.scalar_type() && o.sizes() == x.sizes() &&
+                  (V == 1 || o.stride(1) == 1) && (T <= 1 || o.stride(0) >= V),
+              op, ": out must have the logits' type, shape and device, unit inner stride and rows of their own");
+  if (T == 0) return;
+  const int64_t es = x.element_size(), lx = T > 1 ? x.stride(0) : V, lo = T > 1 ? o.stride(0) : V;
+  const char *xb = (const char*)x.data_ptr(), *ob = (const char*)o.data_ptr();
+  const char *xe = xb + ((T - 1) * lx + V) * es, *oe = ob + ((T - 1) * lo + V) * es;
+  bool ok = xe <= ob || oe <= xb || (xb == ob && lx == lo);
+  if (!ok && lx == lo && (ob - xb) % es == 0) {      // columns of one buffer, side by side
+    const int64_t d = (((ob - xb) / es) % lx + lx) % lx;
+    ok = d >= V && d <= lx - V;
+  }
+  TORCH_CHECK(ok, op, ": out overlaps the logits without being them");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(const at::Tensor& x,
+                                                                                      const at::Tensor& tokens,
+                                                                                      double temperature, int64_t top,
+                                                                                      int64_t ignore_index) {
+  const char* op = "token_logprobs";
+  const int dt = check_logits(x, op);
+  check_temperature(temperature, op);
+  TORCH_CHECK(top >= 0 && top <= x.size(1) && top <= kf_token_logprobs_top_max(), op, ": top must be 0 to ",
+              kf_token_logprobs_top_max(), " and at most V");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(x.device());
+  const auto tok = check_tokens(tokens, x, op);
+  const int64_t T = x.size(0);
+  auto f32 = x.options().dtype(at::kFloat);
+  auto logp = at::empty({T}, f32), entropy = at::empty({T}, f32), stats = at::empty({T, 2}, f32);
+  auto ids = at::empty({T, top}, x.options().dtype(at::kLong)), tlp = at::empty({T, top}, f32);
+  check_rc(kf_token_logprobs(x.data_ptr(), dt, x.stride(0), T, (int)x.size(1), tok.data_ptr<int64_t>(), ignore_index,
+                             (float)temperature, logp.data_ptr<float>(), entropy.data_ptr<float>(),
+                             stats.data_ptr<float>(), (int)top, ids.data_ptr<int64_t>(), tlp.data_ptr<float>(),
+                             cur_stream()),
+           op);
+  return {logp, entropy, stats, ids, tlp};
+}
+
+void token_logprobs_bwd(const at::Tensor& x, const at::Tensor& tokens, const at::Tensor& stats,
+                        const at::Tensor& entropy, const std::optional<at::Tensor>& dlogp,
+                        const std::optional<at::Tensor>& dentropy, double temperature, int64_t ignore_index,
+                        at::Tensor d) {
+  const char* op = "token_logprobs_bwd";
+  const int dt = check_logits(x, op);
+  check_temperature(temperature, op);
+  check_rows_f32(stats, x, 2, op, "stats");
+  check_rows_f32(entropy, x, 0, op, "entropy");
+  if (dlogp.has_value()) check_rows_f32(*dlogp, x, 0, op, "dlogp");
+  if (dentropy.has_value()) check_rows_f32(*dentropy, x, 0, op, "dentropy");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(x.device());
+  const auto tok = check_tokens(tokens, x, op);
+  check_grad_out(x, d, op);
+  check_rc(kf_token_logprobs_bwd(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), x.size(0), (int)x.size(1),
+                                 tok.data_ptr<int64_t>(), ignore_index, stats.data_ptr<float>(),
+                                 entropy.data_ptr<float>(), dlogp.has_value() ? dlogp->data_ptr<float>() : nullptr,
+                                 dentropy.has_value() ? dentropy->data_ptr<float>() : nullptr, (float)temperature,
+                                 cur_stream()),
+           op);
+}
+
+// mode 0: loss rows, gradient into out; 1: loss rows and this part's statistics [T, 5]; 2: loss rows
+// from joined statistics [T, 4] (or one undivided part's [T, 5]), gradient into out
+std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& z,
+                                                const std::optional<at::Tensor>& lse, double temperature,
+                                                const std::optional<at::Tensor>& scale, double scale_h,
+                                                const std::optional<at::Tensor>& rows, int64_t vocab_start,
+                                                int64_t vocab_size, int64_t mode,
+                                                const std::optional<at::Tensor>& stats_in,
+                                                const std::optional<at::Tensor>& out) {
+  const char* op = "distill_topk";
+  const int dt = check_logits(x, op);
+  check_temperature(temperature, op);
+  const int64_t T = x.size(0), V = x.size(1);
+  TORCH_CHECK(ids.device() == x.device() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) &&
+                  ids.dim() == 2 && ids.size(0) == T && (ids.size(1) <= 1 || ids.stride(1) == 1),
+              op, ": ids must be int64 or int32 [T, K] with unit inner stride on the logits' device");
+  const int64_t K = ids.size(1);
+  TORCH_CHECK(K <= kf_distill_k_max(), op, ": at most ", kf_distill_k_max(), " entries a row");
+  const int zt = float_type(z, op, "teacher logits");
+  TORCH_CHECK(z.device() == x.device() && z.sizes() == ids.sizes() && (K <= 1 || z.stride(1) == 1), op,
+              ": teacher logits must be [T, K] with unit inner stride on the logits' device");
+  if (lse.has_value()) {
+    check_rows_f32(*lse, x, 0, op, "lse");
+    TORCH_CHECK(V <= kf_distill_rest_v_max(), op, ": with a teacher lse at most ", kf_distill_rest_v_max(),
+                " logits a row");
+  }
+  TORCH_CHECK(mode >= 0 && mode <= 2, op, ": mode");
+  TORCH_CHECK(vocab_start >= 0 && vocab_size >= vocab_start + V, op, ": the part's logits lie outside the vocabulary");
+  TORCH_CHECK(mode != 0 || vocab_size == V, op, ": a part of a vocabulary goes through statistics and gradient");
+  if (scale.has_value())
+    TORCH_CHECK(scale->device() == x.device() && scale->scalar_type() == at::kFloat && scale->numel() == 1, op,
+                ": scale must be a number or one float32 on the logits' device");
+  if (rows.has_value()) check_rows_f32(*rows, x, 0, op, "row weights");
+  c10::hip::HIPGuardMasqueradingAsCUDA g(x.device());
+  auto f32 = x.options().dtype(at::kFloat);
+  auto loss = at::empty({T}, f32);
+  auto part = at::empty({mode == 1 ? T : 0, 5}, f32);
+  float* st = mode == 1 ? part.data_ptr<float>() : nullptr;
+  int64_t ld_stats = 5;
+  if (mode == 2) {
+    TORCH_CHECK(stats_in.has_value(), op, ": joined statistics required");
+    check_rows_f32(*stats_in, x, stats_in->dim() == 2 && stats_in->size(1) == 5 ? 5 : 4, op, "stats");
+    st = stats_in->data_ptr<float>();
+    ld_stats = stats_in->size(1);
+  }
+  TORCH_CHECK((mode == 1) != out.has_value(), op, ": out goes with a gradient");
+  if (out.has_value()) check_grad_out(x, *out, op);
+  check_rc(kf_distill_topk(x.data_ptr(), dt, x.stride(0), out.has_value() ? out->data_ptr() : nullptr,
+                           out.has_value() ? out->stride(0) : 0, T, (int)V, vocab_start, vocab_size, ids.data_ptr(),
+                           ids.scalar_type() == at::kInt ? 1 : 0, ids.stride(0), z.data_ptr(), zt, z.stride(0),
+                           lse.has_value() ? lse->data_ptr<float>() : nullptr, (int)K, (float)temperature,
+                           scale.has_value() ? scale->data_ptr<float>() : nullptr, (float)scale_h,
+                           rows.has_value() ? rows->data_ptr<float>() : nullptr, loss.data_ptr<float>(), st, ld_stats, (int)mode,
+                           cur_stream()),
+           op);
+  return {loss, part};
 }
 
 // ---------------- Flash attention (K3) ----------------
@@ -827,6 +988,13 @@ TORCH_LIBRARY(kfamd, m) {
   m.def("shard_sum_(Tensor recv, int R, Tensor(a!) out, bool accumulate) -> ()", &shard_sum_);
   m.def("grad_accum_(Tensor(a!) main, Tensor(b!) g, int mode) -> ()", &grad_accum_);
   m.def("cross_entropy_", &cross_entropy_);
+  m.def("token_logprobs(Tensor logits, Tensor tokens, float temperature, int top, int ignore_index) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor)", &token_logprobs);
+  m.def("token_logprobs_bwd(Tensor logits, Tensor tokens, Tensor stats, Tensor entropy, Tensor? dlogp, Tensor? dentropy, "
+        "float temperature, int ignore_index, Tensor(a!) out) -> ()", &token_logprobs_bwd);
+  m.def("distill_topk(Tensor logits, Tensor ids, Tensor z, Tensor? lse, float temperature, Tensor? scale, float scale_h, "
+        "Tensor? rows, int vocab_start, int vocab_size, int mode, Tensor? stats, Tensor(a!)? out) -> (Tensor, Tensor)",
+        &distill_topk);
   m.def("flash_fwd", &flash_fwd);
   m.def("flash_bwd", &flash_bwd);
   m.def("decode_attn", &decode_attn);

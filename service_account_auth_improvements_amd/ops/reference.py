@@ -92,6 +92,170 @@ def cross_entropy(logits, labels, ignore_index=-100, scale=None):
     return loss, lse, p
 
 
+FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+TOP_MAX, DISTILL_K_MAX, DISTILL_REST_V_MAX = 128, 256, 491520    # the GPU kernels' limits
+
+
+def _need(ok, msg):
+    if not ok:
+        raise RuntimeError(msg)
+
+
+def _check_logits(x, temperature, op):
+    _need(x.dtype in FLOATS, f"{op}: logits must be bfloat16, float16 or float32")
+    _need(x.dim() == 2 and x.shape[1] >= 1 and (x.shape[1] == 1 or x.stride(1) == 1),
+          f"{op}: logits must be [T, V] with V >= 1 and unit inner stride")
+    _need(1e-4 <= temperature <= 1e4, f"{op}: temperature must be between 1e-4 and 1e4")
+
+
+def _check_tokens(tokens, x, op):
+    _need(tokens.device == x.device and tokens.dtype == torch.int64 and tuple(tokens.shape) == (x.shape[0],),
+          f"{op}: tokens must be int64 [T] on the logits' device")
+
+
+def _check_rows(t, x, tail, op, name):
+    _need(t.device == x.device and t.dtype == torch.float32 and t.is_contiguous()
+          and tuple(t.shape) == (x.shape[0], *tail), f"{op}: {name} must be contiguous float32 on the logits' device")
+
+
+def _check_out(out, x, op):
+    _need(out.device == x.device and out.dtype == x.dtype and out.shape == x.shape
+          and (x.shape[1] == 1 or out.stride(1) == 1) and (x.shape[0] <= 1 or out.stride(0) >= x.shape[1]),
+          f"{op}: out must have the logits' type, shape and device, unit inner stride and rows of their own")
+
+
+def token_logprobs(logits, tokens, temperature=1.0, top=0, ignore_index=-100):
+    """(logp, entropy, stats [T, 2] = (max, log2 of the sum), top ids, top logp): ops.token_logprobs_fwd."""
+    op = "token_logprobs"
+    _check_logits(logits, temperature, op)
+    _need(0 <= top <= min(TOP_MAX, logits.shape[1]), f"{op}: top must be 0 to {TOP_MAX} and at most V")
+    _check_tokens(tokens, logits, op)
+    V = logits.shape[1]
+    x = logits.float()
+    m = x.amax(1, keepdim=True)
+    d = x - m
+    e = torch.exp(d / temperature)
+    s = e.sum(1, keepdim=True)
+    logs = torch.log(s)
+    lp = d / temperature - logs
+    dead = tokens == ignore_index
+    bad = ~dead & ((tokens < 0) | (tokens >= V))
+    logp = lp.gather(1, tokens.clamp(0, V - 1).unsqueeze(1)).squeeze(1)
+    logp = logp.masked_fill(bad, float("nan")).masked_fill(dead, 0.0)
+    p = e / s
+    ent = -torch.where(p == 0, p, p * lp).sum(1).masked_fill(dead, 0.0)
+    stats = torch.cat([m, logs / math.log(2.0)], 1).masked_fill(dead.unsqueeze(1), 0.0)
+    # NaN first, then descending, equal values (-0 and +0 too) by ascending id
+    ids = torch.sort(x + 0.0, dim=1, descending=True, stable=True).indices[:, :top]
+    tlp = lp.gather(1, ids).masked_fill(dead.unsqueeze(1), 0.0)
+    return logp, ent, stats, ids.masked_fill(dead.unsqueeze(1), -1), tlp
+
+
+def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperature, ignore_index, out):
+    op = "token_logprobs_bwd"
+    _check_logits(logits, temperature, op)
+    _check_tokens(tokens, logits, op)
+    _check_rows(stats, logits, (2,), op, "stats")
+    _check_rows(entropy, logits, (), op, "entropy")
+    for t, name in ((dlogp, "dlogp"), (dentropy, "dentropy")):
+        if t is not None:
+            _check_rows(t, logits, (), op, name)
+    _check_out(out, logits, op)
+    V = logits.shape[1]
+    z = torch.zeros(logits.shape[0], 1)
+    g = z if dlogp is None else dlogp.unsqueeze(1)
+    h = z if dentropy is None else dentropy.unsqueeze(1)
+    lp = (logits.float() - stats[:, :1]) / temperature - stats[:, 1:] * math.log(2.0)
+    p = torch.exp(lp)
+    d = -g * p - h * torch.where(p == 0, p, p * (lp + entropy.unsqueeze(1)))
+    d.scatter_add_(1, tokens.clamp(0, V - 1).unsqueeze(1), g)
+    dead = tokens == ignore_index
+    bad = ~dead & ((tokens < 0) | (tokens >= V))
+    d = (d / temperature).masked_fill(bad.unsqueeze(1), float("nan")).masked_fill(dead.unsqueeze(1), 0.0)
+    return out.copy_(d)
+
+
+def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_start, vocab_size, mode, stats, out):
+    """ops.distill_topk_*: mode 0 loss rows and gradient; 1 loss rows and statistics [T, 5]; 2 loss rows
+    and gradient from joined statistics [T, 4].  Returns (loss, statistics)."""
+    op = "distill_topk"
+    _check_logits(logits, temperature, op)
+    T, V = logits.shape
+    _need(ids.device == logits.device and ids.dtype in (torch.int64, torch.int32) and ids.dim() == 2
+          and ids.shape[0] == T and (ids.shape[1] <= 1 or ids.stride(1) == 1),
+          f"{op}: ids must be int64 or int32 [T, K] with unit inner stride on the logits' device")
+    _need(ids.shape[1] <= DISTILL_K_MAX, f"{op}: at most {DISTILL_K_MAX} entries a row")
+    _need(z.dtype in FLOATS, f"{op}: teacher logits must be bfloat16, float16 or float32")
+    _need(z.device == logits.device and z.shape == ids.shape and (z.shape[1] <= 1 or z.stride(1) == 1),
+          f"{op}: teacher logits must be [T, K] with unit inner stride on the logits' device")
+    if lse is not None:
+        _check_rows(lse, logits, (), op, "lse")
+        _need(V <= DISTILL_REST_V_MAX, f"{op}: with a teacher lse at most {DISTILL_REST_V_MAX} logits a row")
+    _need(vocab_start >= 0 and vocab_size >= vocab_start + V, f"{op}: the part's logits lie outside the vocabulary")
+    _need(mode != 0 or vocab_size == V, f"{op}: a part of a vocabulary goes through statistics and gradient")
+    if scale is not None:
+        _need(scale.device == logits.device and scale.dtype == torch.float32 and scale.numel() == 1,
+              f"{op}: scale must be a number or one float32 on the logits' device")
+        scale_h = float(scale.reshape(-1)[0])
+    if rows is not None:
+        _check_rows(rows, logits, (), op, "row weights")
+    if mode == 2:
+        _check_rows(stats, logits, (5,) if tuple(stats.shape[1:]) == (5,) else (4,), op, "stats")
+    if out is not None:
+        _check_out(out, logits, op)
+    nan, zero = float("nan"), torch.zeros(())
+    ids = ids.long()
+    has = ids >= 0
+    bad = (ids >= vocab_size).any(1)
+    here = (ids >= vocab_start) & (ids < vocab_start + V)
+    col = torch.where(here, ids - vocab_start, V)                      # V: a column that is cut off again
+    zt = torch.where(has, z.float() / temperature, float("-inf"))
+    if lse is None:
+        mz = zt.amax(1, keepdim=True) if zt.shape[1] else torch.full((T, 1), float("-inf"))
+        mz = torch.where(torch.isneginf(mz), 0.0, mz)
+        q = torch.exp(zt - mz)
+        n = q.sum(1, keepdim=True)
+        lq = zt - mz - torch.log(n)
+        q = torch.where(n == 0, n, q / n)
+        rest = torch.zeros(T)
+    else:
+        lq = zt - lse.unsqueeze(1)
+        q = torch.where(has, torch.exp(lq), zero)
+        rest = (1 - q.sum(1)).clamp(min=0)
+    some = (q != 0).any(1)
+    W = (q.sum(1) + rest).unsqueeze(1)
+    x = logits.float()
+    inside = torch.zeros(T, V + 1, dtype=torch.bool).scatter_(1, col, True)[:, :V]
+    xk = torch.cat([x, torch.zeros(T, 1)], 1).gather(1, col)
+    if mode != 2:
+        m = x.amax(1, keepdim=True)
+        d = torch.where(torch.isneginf(m), x, x - m)
+        e = torch.exp(d / temperature)
+        s, u = e.sum(1, keepdim=True), torch.where(inside, zero, e).sum(1, keepdim=True)
+        if lse is None:
+            u = torch.zeros_like(s)
+        ok = here & (q != 0)
+        xq = torch.where(ok, q * (xk - m), zero).sum(1, keepdim=True)
+        part = torch.cat([m, s, u, xq, torch.where(here, q, zero).sum(1, keepdim=True)], 1)
+    else:
+        m, s, u, xq = stats[:, :4].split(1, 1)
+        part = None
+    logs = torch.log(s)
+    live = (rest.unsqueeze(1) > 0) & (u != 0)
+    loss = torch.where(q != 0, q * (lq + logs), zero).sum(1) - (xq / temperature).squeeze(1)
+    r1 = rest.unsqueeze(1)
+    loss = loss + torch.where(live, r1 * (torch.log(r1) - (torch.log(u) - logs)), zero).squeeze(1)
+    loss = loss.masked_fill(~some, 0.0).masked_fill(bad, nan)
+    if mode == 1:
+        return loss, part.masked_fill(~some.unsqueeze(1), 0.0).masked_fill(bad.unsqueeze(1), nan)
+    p = torch.exp((x - m) / temperature - logs)
+    dx = torch.where(inside, p * W, p * torch.where(live, W - r1 * s / u, W))
+    dx = torch.cat([dx, torch.zeros(T, 1)], 1).scatter_add_(1, col, torch.where(here, -q, zero))[:, :V]
+    dx = dx * (scale_h / temperature) * (1.0 if rows is None else rows.unsqueeze(1))
+    out.copy_(dx.masked_fill(~some.unsqueeze(1), 0.0).masked_fill(bad.unsqueeze(1), nan))
+    return loss, None
+
+
 def adamw_(p, w, m, v, g, n_decay, lr, b1, b2, eps, wd, step, gscale=1.0, sumsq=None,
            max_norm=0.0):
     gf = g.float() * gscale
