@@ -349,20 +349,21 @@ def distill_topk_fused(logits, teacher_ids, teacher_logits, scale, temperature=1
 def distill_topk_stats(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None, vocab_start=0,
                        vocab_size=None):
     """:func:`distill_topk_fused` of one vocabulary part (columns [vocab_start, vocab_start + V) of
-    ``vocab_size``; the teacher's ids are global), first half: this part's row statistics [T, 5].
+    ``vocab_size``; the teacher's ids are global), first half: this part's row statistics [T, 8].
     Join the parts' with :func:`distill_topk_join`, then :func:`distill_topk_grad`."""
     return _distill(logits, teacher_ids, teacher_logits, teacher_lse, temperature, 1.0, None, vocab_start, vocab_size,
                     DISTILL_STATS, None, None)[1]
 
 
 def distill_topk_join(parts, temperature=1.0):
-    """Statistics [R, T, 5] of the R parts of a vocabulary -> the whole rows' [T, 4]."""
-    m, s, u, xq, q = parts.unbind(-1)
+    """Statistics [R, T, 8] of the R parts of a vocabulary -> the whole rows' [T, 8]."""
+    m, s, u, xq, q = parts[..., :5].unbind(-1)
     M = m.amax(0)
     # a part (or row) of nothing but -inf: its sums are 0 whatever the shift
     d = torch.where(torch.isneginf(m) | (m == M), torch.zeros_like(m), m - M)
     f = torch.exp(d / temperature)
-    return torch.stack([M, (s * f).sum(0), (u * f).sum(0), (xq + torch.where(q == 0, q, q * d)).sum(0)], -1)
+    student = torch.stack([M, (s * f).sum(0), (u * f).sum(0), (xq + torch.where(q == 0, q, q * d)).sum(0), q.sum(0)], -1)
+    return torch.cat([student, parts[0, :, 5:]], -1)          # the teacher's columns are the same everywhere
 
 
 def distill_topk_grad(logits, teacher_ids, teacher_logits, stats, scale, temperature=1.0, teacher_lse=None,

@@ -69,14 +69,17 @@ int kf_gemm_tn2(const void*, long, const void*, long, void*, long, int, int, con
                 long, int, int, int, int, hipStream_t);
 int kf_transpose_bf16(const void*, long, void*, long, int, int, hipStream_t);
 int kf_token_logprobs_top_max();
+long kf_token_logprobs_scratch(int, long, int, int);
 int kf_token_logprobs(const void*, int, long, long, int, const long*, long, float, float*, float*, float*, int, long*,
-                      float*, hipStream_t);
+                      float*, void*, hipStream_t);
 int kf_token_logprobs_bwd(const void*, int, long, void*, long, long, int, const long*, long, const float*, const float*,
                           const float*, const float*, float, hipStream_t);
 int kf_distill_k_max();
+int kf_distill_stats_cols();
+int kf_distill_needs_stats(int, int);
 long kf_distill_rest_v_max();
 int kf_distill_topk(const void*, int, long, void*, long, long, int, long, long, const void*, int, long, const void*, int,
-                    long, const float*, int, float, const float*, float, const float*, float*, float*, long, int, hipStream_t);
+                    long, const float*, int, float, const float*, float, const float*, float*, float*, int, hipStream_t);
 long kf_car_header_bytes();
 int kf_car_alloc(long, void**, void*);
 int kf_car_open(const void*, void**);
@@ -352,10 +355,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log
   auto f32 = x.options().dtype(at::kFloat);
   auto logp = at::empty({T}, f32), entropy = at::empty({T}, f32), stats = at::empty({T, 2}, f32);
   auto ids = at::empty({T, top}, x.options().dtype(at::kLong)), tlp = at::empty({T, top}, f32);
+  // few rows: several blocks work on one, through scratch of this call's own
+  const int64_t scratch_bytes = kf_token_logprobs_scratch(dt, T, (int)x.size(1), (int)top);
+  at::Tensor scratch;
+  if (scratch_bytes > 0) scratch = at::empty({scratch_bytes / 4}, f32);
   check_rc(kf_token_logprobs(x.data_ptr(), dt, x.stride(0), T, (int)x.size(1), tok.data_ptr<int64_t>(), ignore_index,
                              (float)temperature, logp.data_ptr<float>(), entropy.data_ptr<float>(),
                              stats.data_ptr<float>(), (int)top, ids.data_ptr<int64_t>(), tlp.data_ptr<float>(),
-                             cur_stream()),
+                             scratch_bytes > 0 ? scratch.data_ptr() : nullptr, cur_stream()),
            op);
   return {logp, entropy, stats, ids, tlp};
 }
@@ -382,8 +389,8 @@ void token_logprobs_bwd(const at::Tensor& x, const at::Tensor& tokens, const at:
            op);
 }
 
-// mode 0: loss rows, gradient into out; 1: loss rows and this part's statistics [T, 5]; 2: loss rows
-// from joined statistics [T, 4] (or one undivided part's [T, 5]), gradient into out
+// mode 0: loss rows, gradient into out; 1: loss rows of an undivided vocabulary and this part's
+// statistics [T, 8]; 2: loss rows from joined statistics, gradient into out
 std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& z,
                                                 const std::optional<at::Tensor>& lse, double temperature,
                                                 const std::optional<at::Tensor>& scale, double scale_h,
@@ -418,14 +425,14 @@ std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::T
   c10::hip::HIPGuardMasqueradingAsCUDA g(x.device());
   auto f32 = x.options().dtype(at::kFloat);
   auto loss = at::empty({T}, f32);
-  auto part = at::empty({mode == 1 ? T : 0, 5}, f32);
-  float* st = mode == 1 ? part.data_ptr<float>() : nullptr;
-  int64_t ld_stats = 5;
+  const int64_t cols = kf_distill_stats_cols();
+  const bool own_stats = mode == 1 || (mode == 0 && kf_distill_needs_stats(dt, (int)V));
+  auto part = at::empty({own_stats ? T : 0, cols}, f32);
+  float* st = own_stats ? part.data_ptr<float>() : nullptr;
   if (mode == 2) {
     TORCH_CHECK(stats_in.has_value(), op, ": joined statistics required");
-    check_rows_f32(*stats_in, x, stats_in->dim() == 2 && stats_in->size(1) == 5 ? 5 : 4, op, "stats");
+    check_rows_f32(*stats_in, x, cols, op, "stats");
     st = stats_in->data_ptr<float>();
-    ld_stats = stats_in->size(1);
   }
   TORCH_CHECK((mode == 1) != out.has_value(), op, ": out goes with a gradient");
   if (out.has_value()) check_grad_out(x, *out, op);
@@ -434,7 +441,7 @@ std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::T
                            ids.scalar_type() == at::kInt ? 1 : 0, ids.stride(0), z.data_ptr(), zt, z.stride(0),
                            lse.has_value() ? lse->data_ptr<float>() : nullptr, (int)K, (float)temperature,
                            scale.has_value() ? scale->data_ptr<float>() : nullptr, (float)scale_h,
-                           rows.has_value() ? rows->data_ptr<float>() : nullptr, loss.data_ptr<float>(), st, ld_stats, (int)mode,
+                           rows.has_value() ? rows->data_ptr<float>() : nullptr, loss.data_ptr<float>(), st, (int)mode,
                            cur_stream()),
            op);
   return {loss, part};

@@ -176,8 +176,8 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperat
 
 
 def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_start, vocab_size, mode, stats, out):
-    """ops.distill_topk_*: mode 0 loss rows and gradient; 1 loss rows and statistics [T, 5]; 2 loss rows
-    and gradient from joined statistics [T, 4].  Returns (loss, statistics)."""
+    """ops.distill_topk_*: mode 0 loss rows and gradient; 1 loss rows and statistics [T, 8]; 2 loss rows
+    and gradient from joined statistics.  Returns (loss, statistics)."""
     op = "distill_topk"
     _check_logits(logits, temperature, op)
     T, V = logits.shape
@@ -200,7 +200,7 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
     if rows is not None:
         _check_rows(rows, logits, (), op, "row weights")
     if mode == 2:
-        _check_rows(stats, logits, (5,) if tuple(stats.shape[1:]) == (5,) else (4,), op, "stats")
+        _check_rows(stats, logits, (8,), op, "stats")
     if out is not None:
         _check_out(out, logits, op)
     nan, zero = float("nan"), torch.zeros(())
@@ -236,7 +236,10 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
             u = torch.zeros_like(s)
         ok = here & (q != 0)
         xq = torch.where(ok, q * (xk - m), zero).sum(1, keepdim=True)
-        part = torch.cat([m, s, u, xq, torch.where(here, q, zero).sum(1, keepdim=True)], 1)
+        # the student's (max, sum, outside sum, sum q (x - max), sum q here), the teacher's (max and sum
+        # of the softmax, or 0 and sum q) and whether the row has entries
+        tm, tn = (mz * temperature, n) if lse is None else (torch.zeros(T, 1), q.sum(1, keepdim=True))
+        part = torch.cat([m, s, u, xq, torch.where(here, q, zero).sum(1, keepdim=True), tm, tn, torch.ones(T, 1)], 1)
     else:
         m, s, u, xq = stats[:, :4].split(1, 1)
         part = None

@@ -136,6 +136,15 @@ def test_top_alternatives_in_an_order_that_meets_the_stride(V, group, top, great
     _check_fwd(x, _tok(2, V), 1.0, top)
 
 
+@pytest.mark.parametrize("T", [1, 2, 31, 100, 255, 256, 257])
+def test_few_and_many_rows(T):
+    """Rows that several blocks share and rows of one block."""
+    for V, top in ((20001, 0), (20001, 11), (4104, 128), (65537, 3)):
+        x, tok = _x(T, V, BF16, 0, 1), _tok(T, V)
+        tok[T // 2] = -100 if T > 2 else tok[T // 2]
+        _check_fwd(x, tok, 0.9, top)
+
+
 def test_logprobs_expanded_and_broadcast_inputs():
     x = _x(1, 3001, BF16).expand(7, 3001)                    # row stride 0
     tok = _tok(7, 3001)
@@ -273,6 +282,44 @@ def test_distill_in_vocabulary_parts(dtype, lse):
         loss, d = ops.distill_topk_grad(x[:, a:b], ids, z, joined, 2.0, temp, L, a, V)
         oracle.close(loss, rl, (1 + lsize) * 8 * oracle.sum_bound(V), "loss")
         oracle.close(d, 2 * rd[:, a:b], oracle.grad_bound(2 * rd[:, a:b], 2 * size[:, a:b], 60.0, V, dtype), "dlogits")
+
+
+@pytest.mark.parametrize("lse", [False, True])
+@pytest.mark.parametrize("T,V,dtype", [(700, 65601, BF16), (1200, 40000, FP16), (2100, 3001, BF16), (600, 40000, F32), (40, 262145, BF16)])
+def test_distill_more_rows_than_blocks(T, V, dtype, lse):
+    """Blocks that walk several rows: each row's result is the one it has alone, and the sampled ones the oracle's."""
+    x = _x(T, V, dtype, 0, 3, 1)
+    K = 20
+    g = torch.Generator().manual_seed(4)
+    ids = (torch.randint(0, V, (T, 1), generator=g) + torch.randint(1, V // K, (T, 1), generator=g) * torch.arange(K)) % V
+    ids[::7] = -1
+    ids[3::11, 5:] = -1
+    z = torch.randn(T, K, generator=g) * 2
+    L = torch.logsumexp(z, 1) + 0.1 if lse else None
+    dev = lambda t: None if t is None else t.to(DEV)          # noqa: E731
+    loss, d = ops.distill_topk_fused(x, dev(ids), dev(z), 0.5, 1.0, dev(L))
+    for rows in ([0, 1, T // 2, T - 1], [255 % T, 256 % T, 257 % T, 511 % T, 512 % T]):
+        sel = lambda t: None if t is None else t[rows]        # noqa: E731
+        lo, da = ops.distill_topk_fused(x[rows], dev(ids[rows]), dev(z[rows]), 0.5, 1.0, dev(sel(L)))
+        assert torch.equal(lo, loss[rows]) and torch.equal(da, d[rows])
+    rows = [0, 1, 3, T // 2, T - 1]
+    rl, rd, size, lsize = oracle.distill(x[rows].cpu(), ids[rows], z[rows], 1.0, None if L is None else L[rows])
+    oracle.close(loss[rows], rl, (1 + lsize) * 4 * oracle.sum_bound(V), "loss")
+    oracle.close(d[rows], rd * 0.5, oracle.grad_bound(rd * 0.5, size * 0.5, 60.0, V, dtype), "dlogits")
+
+
+def test_distill_empty_rows_of_nan_logits():
+    """A row without targets is 0 whatever its logits hold."""
+    for V in (500, 40000, 300001):
+        x = _x(3, V, F32)
+        x[1], x[2] = float("nan"), float("inf")
+        ids = torch.zeros(3, 4, dtype=torch.long, device=DEV)
+        ids[1] = -1
+        z = torch.randn(3, 4, device=DEV)
+        z[2] = NEG
+        for L in (None, torch.full((3,), 3.0, device=DEV)):
+            loss, d = ops.distill_topk_fused(x, ids, z, 1.0, 1.0, L)
+            assert torch.isfinite(loss).all() and (loss[1:] == 0).all() and (d[1:] == 0).all() and torch.isfinite(d).all()
 
 
 def test_teacher_to_student_run():
