@@ -90,7 +90,7 @@ def build_ops_check(force: bool = False, jobs: int | None = None) -> Path:
     import torch
     import torch.utils.cpp_extension as ce
 
-    from ..ops._build import FILE_FLAGS, NO_PACKED_F32
+    from ..ops._build import FILE_FLAGS
 
     inc = ce.include_paths(device_type="cuda")
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -99,7 +99,7 @@ def build_ops_check(force: bool = False, jobs: int | None = None) -> Path:
             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
             "-Wno-unused-result", "-Wno-deprecated-declarations"]
     # .hip sources: device code for gfx950 as usual, sanitizers on the host pass only
-    hip_flags = base + [f"--offload-arch={ARCH}", "-ffp-contract=fast", "-munsafe-fp-atomics", *NO_PACKED_F32,
+    hip_flags = base + [f"--offload-arch={ARCH}", "-ffp-contract=fast", "-munsafe-fp-atomics",
                         "-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
                         *[x for f in UB_OFF for x in ("-Xarch_host", f)]]
     # host-only C++ (bindings + harness): no device pass at all

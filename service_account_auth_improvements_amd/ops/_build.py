@@ -45,7 +45,7 @@ def _flags():
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-Wno-unused-result", "-Wno-deprecated-declarations",
     ]
-    kernel = common + ["-ffp-contract=fast", "-munsafe-fp-atomics", *NO_PACKED_F32]
+    kernel = common + ["-ffp-contract=fast", "-munsafe-fp-atomics"]
     binding = common + [f"-I{p}" for p in inc] + ["-DTORCH_EXTENSION_NAME=_kfamd_ops",
                                                   "-DHIP_ENABLE_WARP_SYNC_BUILTINS=1"]
     link = ["-shared", "-fPIC", f"--offload-arch={ARCH}", f"-L{lib}", f"-Wl,-rpath,{lib}",
@@ -53,17 +53,19 @@ def _flags():
     return kernel, binding, link
 
 
-# no packed fp32 VALU instructions (v_pk_add/mul/fma_f32) in any kernel: hipcc forms them from
-# ordinary float code, and some of their operand forms have returned wrong values on gfx950.  The
-# host pass does not know the feature and says so; that warning is harmless.
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-
 # per-source extra flags: flash_attn.hip's kernels were tuned (and their code is pinned,
 # tests/test_kernels_static.py) with the MFMA accumulators in the VGPR form, and are built
 # without SLP vectorization: it packed the softmax's f32 adds / multiplies into v_pk_*_f32,
 # which cost more issue slots beside the MFMAs than the scalar ops (attention backward 7.50 ->
 # 7.26 ms at B4 S8192, profiles/fa_fwd128_r5.md)
-FILE_FLAGS = {"flash_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-slp-vectorize"]}
+# The kernels over logits are built without packed fp32 VALU instructions (v_pk_add/mul/fma_f32):
+# hipcc forms them from ordinary float code, and some of their operand forms have returned wrong
+# values on gfx950.  (The host pass does not know the feature and says so; that is harmless.)  The
+# kernels before them keep theirs: without, hipcc contracts other multiply-adds, and trained losses
+# change in the last bits (12.572561 for 12.572235 after one step at Llama-3-8B widths).
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FILE_FLAGS = {"flash_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-slp-vectorize"],
+              "token_logprobs.hip": NO_PACKED_F32, "distill_topk.hip": NO_PACKED_F32}
 
 
 def _sources():
