@@ -34,8 +34,9 @@ constexpr int GROUPS = 256;    // thread groups whose maxima bound the k-th elem
 struct TopShared {
   u32 group[GROUPS];
   alignas(16) u64 cand[CAND + 4];
-  unsigned short who[1024];    // threads with several pieces that reach the bound
-  int nwho, ncand;
+  int alone[1024];             // best pieces of threads where no second one reaches the bound
+  unsigned short who[1024];    // threads with several that do
+  int nalone, nwho, ncand;
   u64 bound;
 };
 
@@ -134,7 +135,7 @@ __device__ __forceinline__ void block_top(const char* row, int V, int p0, int p1
 #pragma unroll
   for (int o = 1; o < PER; o <<= 1) g = max(g, (u32)__shfl_xor((int)g, o, 64));
   if (tid % PER == 0) sh.group[tid / PER] = g;
-  if (tid == 0) sh.nwho = 0;
+  if (tid == 0) sh.nalone = sh.nwho = 0;
   __syncthreads();
   if (tid < 64) {
     const u32 b = wave_kth(sh.group, k);
@@ -143,31 +144,27 @@ __device__ __forceinline__ void block_top(const char* row, int V, int p0, int p1
   __syncthreads();
   u64 bound = sh.bound;                          // 0: fewer than k groups, every element is taken
   const u32 floor = (u32)(bound >> 32);
-  const bool alone = have && mine >= floor && second < floor;
   if (have && second >= floor) sh.who[atomicAdd(&sh.nwho, 1)] = (unsigned short)tid;
-  auto take = [&](int c) {
-    if (*(volatile int*)&sh.ncand > CAND) return;             // too many already: another round
-    float f[N];
-    load_any<DT>(row, c, V, 0.f, f);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const u32 idx = (u32)N * c + j;
-      const u64 key = elem_key(f[j], idx);
-      if (idx < (u32)V && key >= bound) {
-        const int at = atomicAdd(&sh.ncand, 1);
-        if (at < CAND) sh.cand[at] = key;
-      }
-    }
-  };
+  else if (have && mine >= floor) sh.alone[atomicAdd(&sh.nalone, 1)] = best.c;
   for (;;) {
     if (tid == 0) sh.ncand = 0;
     __syncthreads();
-    // a thread reads its own best piece; threads that need more are shared out
-    if (alone) take(best.c);
-    const int nwho = sh.nwho, niter = (p1 - p0 + NT - 1) / NT;
-    for (int w = tid; w < nwho * niter; w += NT) {
-      const int c = p0 + (w / nwho) * NT + sh.who[w % nwho];
-      if (c < p1) take(c);
+    const int nwho = sh.nwho, nall = nwho * ((p1 - p0 + NT - 1) / NT), nwork = nall + sh.nalone;
+    for (int w = tid; w < nwork; w += NT) {
+      const int c = w < nall ? p0 + (w / nwho) * NT + sh.who[w % nwho] : sh.alone[w - nall];
+      // too many already: another round
+      if (c >= p1 || *(volatile int*)&sh.ncand > CAND) continue;
+      float f[N];
+      load_any<DT>(row, c, V, 0.f, f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const u32 idx = (u32)N * c + j;
+        const u64 key = elem_key(f[j], idx);
+        if (idx < (u32)V && key >= bound) {
+          const int at = atomicAdd(&sh.ncand, 1);
+          if (at < CAND) sh.cand[at] = key;
+        }
+      }
     }
     __syncthreads();
     const int n = sh.ncand, held = n < CAND ? n : CAND;
@@ -245,6 +242,11 @@ __device__ __forceinline__ RowStat walk_row(const char* row, int V, int p0, int 
   return st;
 }
 
+// written out, so that a token's log-probability is the same bits as the given one and as an alternative
+__device__ __forceinline__ float ln_p(float x, float m, float L, float inv_temp) {
+  return fmaf(x - m, inv_temp, -__fmul_rn(LN2, L));
+}
+
 struct Result {
   float *logp, *entropy, *stats, *top;
   long* ids;
@@ -254,14 +256,14 @@ __device__ __forceinline__ void write_ignored(const Result& o, long r, int k, in
   for (int i = tid; i < k; i += nt) { o.ids[r * k + i] = -1; o.top[r * k + i] = 0.f; }
 }
 __device__ __forceinline__ void write_row(const Result& o, long r, RowStat st, float L, bool in, float x, float inv_temp) {
-  o.logp[r] = in ? (x - st.m) * inv_temp - LN2 * L : quiet_nan();
+  o.logp[r] = in ? ln_p(x, st.m, L, inv_temp) : quiet_nan();
   o.entropy[r] = LN2 * L - st.u / st.s * inv_temp;
   o.stats[2 * r] = st.m;
   o.stats[2 * r + 1] = L;
 }
 __device__ __forceinline__ void write_top(const Result& o, long r, int k, int rank, u64 key, float m, float L, float inv_temp) {
   o.ids[r * k + rank] = (long)(u32)~(u32)key;
-  o.top[r * k + rank] = (key_value((u32)(key >> 32)) - m) * inv_temp - LN2 * L;
+  o.top[r * k + rank] = ln_p(key_value((u32)(key >> 32)), m, L, inv_temp);
 }
 
 // one block per row; 8 waves a SIMD (registers of both kinds: 100 scalar ones already halve that), so
