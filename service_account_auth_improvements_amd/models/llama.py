@@ -92,6 +92,44 @@ class LlamaConfig:
         return 6 * n_mm + attn
 
 
+class TeacherLogits:
+    """Distillation targets, given in the place of labels to :meth:`Llama.forward_backward`,
+    :meth:`Llama.forward_loss` and the trainers' micro-batches: each token's top logits of a teacher
+    (ops.distill_topk_fused).
+
+    ``ids`` int64 / int32 and ``logits`` [B, S, K]; a token whose ids are all negative is not trained
+    on.  ``lse`` fp32 [B, S]: the log-sum-exp of the teacher's whole rows at ``temperature``, which
+    keeps its remaining mass as one bucket; None renormalises over the K entries.  The loss is the
+    divergence per token in nats, not multiplied by temperature squared (pass that in the scale)."""
+
+    def __init__(self, ids: torch.Tensor, logits: torch.Tensor, temperature: float = 1.0,
+                 lse: Optional[torch.Tensor] = None):
+        if ids.shape != logits.shape or ids.dim() < 2 or (lse is not None and lse.shape != ids.shape[:-1]):
+            raise ValueError("TeacherLogits: ids and logits are [.., K], lse [..]")
+        self.ids, self.logits, self.temperature, self.lse = ids, logits, float(temperature), lse
+
+    def _map(self, f, tail):
+        return TeacherLogits(f(self.ids, tail), f(self.logits, tail), self.temperature,
+                             None if self.lse is None else f(self.lse, ()))
+
+    # what the training code does with labels
+    @property
+    def shape(self):
+        return self.ids.shape[:-1]
+
+    def numel(self) -> int:
+        return self.shape.numel()
+
+    def reshape(self, *shape):
+        return self._map(lambda t, tail: t.reshape(*shape, *tail), (self.ids.shape[-1],))
+
+    def contiguous(self):
+        return self._map(lambda t, tail: t.contiguous(), ())
+
+    def __getitem__(self, index):
+        return self._map(lambda t, tail: t[index], ())
+
+
 def _run(gen):
     """Drive a generator to completion and return its value."""
     while True:
@@ -529,7 +567,10 @@ class Llama:
         return (tot * scale).float()
 
     def _ce_chunk(self, logits, labels, scale):
-        """Cross-entropy of one row chunk: loss rows (fp32); ``logits`` now hold dlogits."""
+        """Cross-entropy (or, for :class:`TeacherLogits`, distillation) of one row chunk: loss rows
+        (fp32); ``logits`` now hold dlogits."""
+        if isinstance(labels, TeacherLogits):
+            return self._distill_chunk(logits, labels, scale)
         if self.tp == 1:
             loss_rows, _ = ops.cross_entropy_fused_(logits, labels, scale)
             return loss_rows
@@ -542,6 +583,18 @@ class Llama:
         lse = M + torch.log(sx[0])
         ops.cross_entropy_grad_(logits, labels, lse, scale, self.vstart)
         return torch.where(labels != -100, lse - sx[1], torch.zeros_like(lse))
+
+    def _distill_chunk(self, logits, t: TeacherLogits, scale):
+        if self.tp == 1:
+            rows, _ = ops.distill_topk_fused(logits, t.ids, t.logits, scale, t.temperature, t.lse, out=logits)
+            return rows
+        part = ops.distill_topk_stats(logits, t.ids, t.logits, t.temperature, t.lse, self.vstart, self.cfg.vocab_size)
+        parts = [torch.empty_like(part) for _ in range(self.tp)]
+        dist.all_gather(parts, part, group=self.st.tp_group)
+        joined = ops.distill_topk_join(torch.stack(parts), t.temperature)
+        rows, _ = ops.distill_topk_grad(logits, t.ids, t.logits, joined, scale, t.temperature, t.lse, self.vstart,
+                                        self.cfg.vocab_size, out=logits)
+        return rows
 
     def head_bwd(self, ctx, accumulate: bool):
         """Row-chunked LM head + CE (K5): per chunk of ``head_chunk`` tokens, logits = y W^T
@@ -705,7 +758,7 @@ class Llama:
     def forward_backward(self, tokens: torch.Tensor, labels: torch.Tensor, accumulate: bool = False,
                          scale: Optional[float] = None):
         """Single-stage fused step: tokens/labels [B, S] -> loss (device scalar); grads
-        written into the flat gradient buffers."""
+        written into the flat gradient buffers.  ``labels`` may be :class:`TeacherLogits`."""
         B, S = tokens.shape
         scale = scale if scale is not None else 1.0 / (B * S)
         loss, ctx = self.stage_forward(tokens.reshape(-1), B, S, labels.reshape(-1), scale)

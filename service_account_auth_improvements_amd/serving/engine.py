@@ -414,12 +414,35 @@ class Request:
     temperature: float = 0.0
     top_p: float = 1.0
     stop: Optional[List[int]] = None
+    # log-probabilities of the output tokens (temperature 1), with this many alternatives each;
+    # None: not computed
+    logprobs: Optional[int] = None
     output: List[int] = field(default_factory=list)
+    token_logprobs: List[float] = field(default_factory=list)
+    top_logprobs: List[List[tuple]] = field(default_factory=list)     # [(token, logprob), ..] per output token
     done: threading.Event = field(default_factory=threading.Event)
     t_submit: float = field(default_factory=time.time)
     t_first: float = 0.0
     t_done: float = 0.0
     error: Optional[str] = None
+
+
+MAX_LOGPROBS = 20             # alternatives a request may ask for
+
+
+def record_logprobs(logits: torch.Tensor, tokens: List[int], reqs: List["Request"]):
+    """Append the log-probability of each request's new token, and its alternatives, for the requests
+    that asked: one ops.token_logprobs_fwd over the batch (the other rows are passed over)."""
+    if all(r.logprobs is None for r in reqs):
+        return
+    top = min(max(r.logprobs or 0 for r in reqs), logits.shape[1])
+    tok = torch.tensor([-100 if r.logprobs is None else t for t, r in zip(tokens, reqs)], dtype=torch.long)
+    logp, _, _, ids, tlp = ops.token_logprobs_fwd(logits, tok.to(logits.device), top=top)
+    logp, ids, tlp = logp.tolist(), ids.tolist(), tlp.tolist()
+    for j, r in enumerate(reqs):
+        if r.logprobs is not None:
+            r.token_logprobs.append(logp[j])
+            r.top_logprobs.append(list(zip(ids[j], tlp[j]))[:r.logprobs])
 
 
 class Scheduler:
@@ -439,6 +462,10 @@ class Scheduler:
     def submit(self, req: Request) -> Request:
         if len(req.prompt) + req.max_new_tokens > self.e.max_len:
             req.error = f"prompt + max_new_tokens exceeds max_len {self.e.max_len}"
+            req.done.set()
+            return req
+        if req.logprobs is not None and not 0 <= req.logprobs <= MAX_LOGPROBS:
+            req.error = f"logprobs must be between 0 and {MAX_LOGPROBS}"
             req.done.set()
             return req
         self.q.put(req)
@@ -466,8 +493,9 @@ class Scheduler:
 
     def _admit_group(self, batch: List[tuple]):
         logits = self.e.prefill_batch([s for s, _ in batch], [r.prompt for _, r in batch])
-        for j, (slot, req) in enumerate(batch):
-            tok = int(sample(logits[j:j + 1], req.temperature, req.top_p)[0])
+        toks = [int(sample(logits[j:j + 1], r.temperature, r.top_p)[0]) for j, (_, r) in enumerate(batch)]
+        record_logprobs(logits, toks, [r for _, r in batch])
+        for tok, (slot, req) in zip(toks, batch):
             req.output.append(tok)
             req.t_first = time.time()
             self.active[slot] = req
@@ -504,6 +532,7 @@ class Scheduler:
             nxt = logits.argmax(-1).tolist()
         else:
             nxt = [int(sample(logits[j:j + 1], r.temperature, r.top_p)[0]) for j, r in enumerate(reqs)]
+        record_logprobs(logits, nxt, reqs)
         self.steps += 1
         for s, r, t in zip(slots, reqs, nxt):
             r.output.append(t)

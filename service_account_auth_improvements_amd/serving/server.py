@@ -8,7 +8,8 @@ Endpoints (KServe v1 / Open Inference Protocol v2 / OpenAI-style completions):
   "max_new_tokens", "temperature", "top_p"}]}`` -> ``{"predictions": [...]}``
 * ``POST /v2/models/<name>/infer`` with a ``BYTES`` ``text_input`` or ``INT64`` ``input_ids``
   tensor -> ``text_output`` / ``output_ids``
-* ``POST /v1/completions`` ``{"prompt", "max_tokens", "temperature", "top_p"}``
+* ``POST /v1/completions`` ``{"prompt", "max_tokens", "temperature", "top_p", "logprobs"}``;
+  ``logprobs`` (0 to 20) adds each output token's log-probability and that many alternatives
 * ``GET /metrics`` (prometheus: request count/latency, tokens generated, TTFT)
 
 Text is tokenised with a HuggingFace ``tokenizer.json`` when ``--tokenizer`` points at one
@@ -18,14 +19,16 @@ the random-init benchmark model can be driven end to end without downloads.
 from __future__ import annotations
 
 import argparse
+import itertools
 import json
 import logging
+import math
 import os
 import threading
 import time
 from typing import List, Optional
 
-from .engine import Request, Scheduler, build_engine
+from .engine import MAX_LOGPROBS, Request, Scheduler, build_engine
 
 log = logging.getLogger("predictor")
 
@@ -62,8 +65,9 @@ def create_app(sched: Scheduler, model_name: str, tokenizer=None, registry=None)
     m_tok = Counter("predictor_generated_tokens_total", "generated tokens", registry=reg)
     app = Flask("predictor")
 
-    def run(prompts: List[List[int]], max_new, temperature, top_p, timeout=600.0):
-        reqs = [sched.submit(Request(prompt=p, max_new_tokens=max_new, temperature=temperature, top_p=top_p))
+    def run(prompts: List[List[int]], max_new, temperature, top_p, timeout=600.0, logprobs=None):
+        reqs = [sched.submit(Request(prompt=p, max_new_tokens=max_new, temperature=temperature, top_p=top_p,
+                                     logprobs=logprobs))
                 for p in prompts]
         for r in reqs:
             if not r.done.wait(timeout):
@@ -168,19 +172,40 @@ def create_app(sched: Scheduler, model_name: str, tokenizer=None, registry=None)
                      "data": [t for r in reqs for t in r.output]}]
         return jsonify({"model_name": model_name, "id": body.get("id", ""), "outputs": outs})
 
+    def logprobs_json(r):
+        """The completions protocol's logprobs object (null where a value is not finite)."""
+        num = lambda v: v if math.isfinite(v) else None      # noqa: E731
+        texts = [tok.decode([t]) for t in r.output]
+        tops = []
+        for alts in r.top_logprobs:
+            d = {}
+            for t, lp in alts:
+                text = tok.decode([t])
+                # ids that decode to the same text keep entries of their own
+                d[text if text and text not in d else f"token_id:{t}"] = num(lp)
+            tops.append(d)
+        return {"tokens": texts, "token_logprobs": [num(v) for v in r.token_logprobs],
+                "top_logprobs": tops if r.logprobs else None,
+                "text_offset": list(itertools.accumulate(map(len, texts[:-1]), initial=0)) if texts else []}
+
     @app.post("/v1/completions")
     def completions():
         body = request.get_json(force=True, silent=True) or {}
         prompt = body.get("prompt", "")
         prompts = prompt if isinstance(prompt, list) else [prompt]
+        logprobs = body.get("logprobs")
+        if logprobs is not None and (type(logprobs) is not int or not 0 <= logprobs <= MAX_LOGPROBS):
+            return jsonify({"error": {"message": f"logprobs must be an integer between 0 and {MAX_LOGPROBS}"}}), 400
         try:
             reqs = run([p if isinstance(p, list) else tok.encode(p) for p in prompts], int(body.get("max_tokens", 16)),
-                       float(body.get("temperature", 0.0)), float(body.get("top_p", 1.0)))
+                       float(body.get("temperature", 0.0)), float(body.get("top_p", 1.0)), logprobs=logprobs)
         except (ValueError, TimeoutError) as e:
             return jsonify({"error": {"message": str(e)}}), 400
         return jsonify({"object": "text_completion", "model": model_name, "created": int(time.time()),
                         "choices": [{"index": i, "text": tok.decode(r.output), "token_ids": r.output,
-                                     "finish_reason": "length"} for i, r in enumerate(reqs)],
+                                     "finish_reason": "length",
+                                     **({} if r.logprobs is None else {"logprobs": logprobs_json(r)})}
+                                    for i, r in enumerate(reqs)],
                         "usage": {"prompt_tokens": sum(len(r.prompt) for r in reqs),
                                   "completion_tokens": sum(len(r.output) for r in reqs)}})
 
