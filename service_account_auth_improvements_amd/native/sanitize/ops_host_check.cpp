@@ -90,6 +90,12 @@ void check_rejections_cpu() {
   expect_reject("cross_entropy_ cpu tensor", "kfamd::cross_entropy_",
                 {lg, lab, 0, -100, c10::IValue(), 1.0, 0, at::zeros({4}, f32), at::zeros({4}, f32), c10::IValue(),
                  c10::IValue(), c10::IValue()});
+  expect_reject("token_logprobs cpu tensor", "kfamd::token_logprobs", {lg, lab, 1.0, 4, -100});
+  expect_reject("token_logprobs_bwd cpu tensor", "kfamd::token_logprobs_bwd",
+                {lg, lab, at::zeros({4, 2}, f32), at::zeros({4}, f32), c10::IValue(), c10::IValue(), 1.0, -100, lg.clone()});
+  expect_reject("distill_topk cpu tensor", "kfamd::distill_topk",
+                {lg, at::zeros({4, 8}, i64), at::zeros({4, 8}, bf), c10::IValue(), 1.0, c10::IValue(), 1.0, c10::IValue(), 0,
+                 512, 0, c10::IValue(), lg.clone()});
   auto qkv = at::randn({128, 3 * 128}, bf);
   expect_reject("flash_fwd cpu tensor", "kfamd::flash_fwd", {qkv, 1, 128, 1, 1, 128, 0.08, true});
   expect_reject("transpose_bf16 cpu tensor", "kfamd::transpose_bf16", {at::randn({64, 64}, bf)});
@@ -214,6 +220,32 @@ void check_gpu() {
     pr.scatter_add_(1, labels.clamp_min(0).unsqueeze(1), -at::ones({T, 1}, f32));
     pr = pr * sc * valid.unsqueeze(1).to(at::kFloat);
     expect_close("cross_entropy_ dlogits", logits, pr, 1e-4, 2e-2);
+  }
+  // token log-probabilities (whole rows and rows shared by blocks), their gradient, distillation
+  for (int64_t V : {(int64_t)4096, (int64_t)40001}) {
+    const int64_t T = 5, K = 12, k = 7;
+    auto x = (at::randn({T, V}, f32) * 3).to(at::kBFloat16);
+    auto tok = at::randint(0, V, {T}, i64);
+    auto lsm = at::log_softmax(x.to(at::kFloat), -1);
+    auto r = call("kfamd::token_logprobs", {x, tok, 1.0, k, -100});
+    auto lp = lsm.gather(1, tok.unsqueeze(1)).squeeze(1), ent = -(lsm.exp() * lsm).sum(-1);
+    expect_close("token_logprobs logp", r[0].toTensor(), lp, 1e-4, 1e-5);
+    expect_close("token_logprobs entropy", r[1].toTensor(), ent, 1e-4, 1e-4);
+    expect_close("token_logprobs alternatives", r[4].toTensor(), std::get<0>(at::topk(lsm, k)), 1e-4, 1e-5);
+    expect_close("token_logprobs ids", lsm.gather(1, r[3].toTensor()), r[4].toTensor(), 1e-4, 1e-5);
+    auto g = at::randn({T}, f32), d = at::empty_like(x);
+    call("kfamd::token_logprobs_bwd", {x, tok, r[2], r[1], g, c10::IValue(), 1.0, -100, d});
+    auto one = at::zeros({T, V}, f32).scatter_(1, tok.unsqueeze(1), at::ones({T, 1}, f32));
+    expect_close("token_logprobs_bwd", d, g.unsqueeze(1) * (one - lsm.exp()), 1e-3, 2e-2);
+    auto ids = std::get<1>(at::topk(at::randn({T, V}, f32), K)), z = at::randn({T, K}, f32);
+    auto q = at::softmax(z, -1);
+    auto l = call("kfamd::distill_topk", {x, ids, z, c10::IValue(), 1.0, c10::IValue(), 1.0, c10::IValue(), 0, V, 0,
+                                          c10::IValue(), d});
+    expect_close("distill_topk loss", l[0].toTensor(), (q * (q.log() - lsm.gather(1, ids))).sum(-1), 1e-4, 1e-5);
+    expect_close("distill_topk dlogits", d, lsm.exp() - at::zeros({T, V}, f32).scatter_(1, ids, q), 1e-3, 2e-2);
+    expect_reject("token_logprobs top > V", "kfamd::token_logprobs", {x.narrow(1, 0, 4), tok, 1.0, 5, -100});
+    expect_reject("distill_topk part as a whole", "kfamd::distill_topk",
+                  {x, ids, z, c10::IValue(), 1.0, c10::IValue(), 1.0, c10::IValue(), 0, 2 * V, 0, c10::IValue(), d});
   }
   // flash attention fwd + bwd (GQA 4:2, causal, two sequences) against fp32 autograd
   {

@@ -291,7 +291,7 @@ def token_logprobs_fwd(logits, tokens, temperature=1.0, top=0, ignore_index=-100
     top_ids [T, top] int64, top_logp [T, top])``, fp32 in nats; ``stats`` is what
     :func:`token_logprobs_bwd` needs.  ``top`` (at most 128 and V) alternatives are ordered by
     descending logit, equal logits by ascending id, NaN first.  Rows whose token is
-    ``ignore_index`` are padding: they are not read, give 0 and ids of -1.  A token outside the
+    ``ignore_index`` are padding: nothing in them counts, and they give 0 and ids of -1.  A token outside the
     vocabulary gives NaN; a row with NaN, with +inf or with nothing but -inf is NaN.  The whole
     vocabulary is expected in one row: under tensor parallelism gather the shards' logits first."""
     if logits.is_cuda:
@@ -306,6 +306,8 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp=None, dentropy=None
     ``out=logits`` overwrites them."""
     if out is None:
         out = logits.new_empty(logits.shape)
+    else:
+        torch.autograd.graph.increment_version(out)
     if logits.is_cuda:
         _k().token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperature, ignore_index, out)
         return out
@@ -317,8 +319,11 @@ DISTILL_FUSED, DISTILL_STATS, DISTILL_GRAD = 0, 1, 2
 
 
 def _distill(logits, ids, z, lse, temperature, scale, rows, vocab_start, vocab_size, mode, stats, out):
-    if mode != DISTILL_STATS and out is None:
-        out = logits.new_empty(logits.shape)
+    if mode != DISTILL_STATS:
+        if out is None:
+            out = logits.new_empty(logits.shape)
+        else:
+            torch.autograd.graph.increment_version(out)
     fn = _k().distill_topk if logits.is_cuda else reference.distill_topk
     st, sh = (scale, 0.0) if torch.is_tensor(scale) else (None, float(scale))
     loss, part = fn(logits, ids, z, lse, temperature, st, sh, rows, vocab_start,
@@ -464,14 +469,16 @@ def swiglu(gu):
 def _refuse_live_leaf(x):
     """A leaf's gradient accumulator belongs to the stream of the first graph that holds it.  A
     backward pass captured on another stream while that graph lives would make the capture wait for
-    work outside it, which ends the process; the forward pass says so instead."""
+    work outside it, which ends the process; the forward pass says so instead.  The accumulator lives
+    as long as a graph holds it, or what this returns."""
     if not (x.is_cuda and x.is_leaf and x.requires_grad and torch.is_grad_enabled()):
-        return
-    seen = torch.autograd.graph.get_gradient_edge(x).node.metadata
+        return None
+    node = torch.autograd.graph.get_gradient_edge(x).node
     stream = torch.cuda.current_stream(x.device).cuda_stream
-    if seen.setdefault("kfamd_stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+    if node.metadata.setdefault("kfamd_stream", stream) != stream and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("these logits are a leaf of an earlier autograd graph that is still alive: drop that "
                            "graph's outputs before capturing, or capture the _fwd / _bwd (or fused) calls")
+    return node
 
 
 class _TokenLogprobsFn(torch.autograd.Function):
@@ -497,7 +504,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
 def token_logprobs(logits, tokens, temperature=1.0, top=0, ignore_index=-100):
     """:func:`token_logprobs_fwd` for autograd: (logp, entropy, top_ids, top_logp); the gradient runs
     through logp and entropy."""
-    _refuse_live_leaf(logits)
+    held = _refuse_live_leaf(logits)      # noqa: F841 -- until the graph holds it
     return _TokenLogprobsFn.apply(logits, tokens, temperature, top, ignore_index)
 
 
@@ -520,5 +527,5 @@ class _DistillTopkFn(torch.autograd.Function):
 
 def distill_topk(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None):
     """:func:`distill_topk_fused`'s loss rows for autograd (the teacher gets no gradient)."""
-    _refuse_live_leaf(logits)
+    held = _refuse_live_leaf(logits)      # noqa: F841 -- until the graph holds it
     return _DistillTopkFn.apply(logits, teacher_ids, teacher_logits, temperature, teacher_lse)

@@ -303,7 +303,7 @@ int float_type(const at::Tensor& t, const char* op, const char* name) {
 int check_logits(const at::Tensor& x, const char* op) {
   TORCH_CHECK(x.is_cuda(), op, ": logits must be a GPU tensor");
   const int dt = float_type(x, op, "logits");
-  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1 && x.size(1) < (1L << 31) - 64 && (x.size(1) == 1 || x.stride(1) == 1), op,
+  TORCH_CHECK(x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= (1L << 31) - 4096 && (x.size(1) == 1 || x.stride(1) == 1), op,
               ": logits must be [T, V] with V >= 1 and unit inner stride");
   return dt;
 }

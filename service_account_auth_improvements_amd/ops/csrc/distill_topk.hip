@@ -355,7 +355,8 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
   const float L = __log2f(st.s);
   // entries of q = 0 add nothing, whatever the student gives them
   const bool use = mine && q != 0.f;
-  const float xq = block_reduce<NT>(use ? q * (x - st.m) : 0.f, 0.f, red[3], OpAdd{}, tid);
+  // (a part of nothing but -inf: its ids' logits, against 0)
+  const float xq = block_reduce<NT>(use ? q * (x - stat_ref(st.m)) : 0.f, 0.f, red[3], OpAdd{}, tid);
   const float ql = block_reduce<NT>(mine ? q : 0.f, 0.f, red[4], OpAdd{}, tid);
   float l = block_reduce<NT>(use ? q * (lq - ((x - st.m) * inv_temp - LN2 * L)) : 0.f, 0.f, red[5], OpAdd{}, tid);
   if (REST && rest > 0.f && !(st.u == 0.f)) l += rest * LN2 * (__log2f(rest) - (__log2f(st.u) - L));

@@ -235,7 +235,7 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
         if lse is None:
             u = torch.zeros_like(s)
         ok = here & (q != 0)
-        xq = torch.where(ok, q * (xk - m), zero).sum(1, keepdim=True)
+        xq = torch.where(ok, q * (xk - torch.where(torch.isneginf(m), 0.0, m)), zero).sum(1, keepdim=True)
         # the student's (max, sum, outside sum, sum q (x - max), sum q here), the teacher's (max and sum
         # of the softmax, or 0 and sum q) and whether the row has entries
         tm, tn = (mz * temperature, n) if lse is None else (torch.zeros(T, 1), q.sum(1, keepdim=True))

@@ -119,6 +119,30 @@ def test_distill_in_vocabulary_parts(cuts, lse):
         oracle.close(d, dw[:, a:b], 64 * oracle.EPS * (1 + dw[:, a:b].abs()), "dlogits")
 
 
+def test_entry_in_a_part_of_nothing_but_minus_infinity():
+    x = _x(2, 20)
+    x[0, :8] = float("-inf")
+    ids, z = torch.tensor([[3, 12], [3, 12]]), torch.zeros(2, 2)
+    whole, dw = ops.distill_topk_fused(x, ids, z, 1.0)
+    st = torch.stack([ops.distill_topk_stats(x[:, a:b].contiguous(), ids, z, 1.0, None, a, 20) for a, b in ((0, 8), (8, 20))])
+    for a, b in ((0, 8), (8, 20)):
+        loss, d = ops.distill_topk_grad(x[:, a:b].contiguous(), ids, z, ops.distill_topk_join(st), 1.0, 1.0, None, a, 20)
+        oracle.close(loss, whole, 64 * oracle.EPS * (1 + whole[1].abs()), "loss")
+        oracle.close(d, dw[:, a:b], 64 * oracle.EPS, "dlogits")
+    assert whole[0] == float("inf")
+
+
+def test_overwritten_logits_are_noticed_by_autograd():
+    x, tok = _x(2, 9), _tok(2, 9)
+    xv = (x.clone().requires_grad_() * 1.0)
+    logp, ent, _, _ = ops.token_logprobs(xv, tok)
+    with torch.no_grad():
+        _, _, st, _, _ = ops.token_logprobs_fwd(xv, tok)
+        ops.token_logprobs_bwd(xv, tok, st, ent.detach(), torch.ones(2), out=xv)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        logp.sum().backward()
+
+
 def test_distill_border_rows():
     # everything covered; student without mass outside; student without mass at an entry; id behind the end
     x = torch.zeros(4, 6)

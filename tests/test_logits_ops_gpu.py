@@ -322,6 +322,19 @@ def test_distill_empty_rows_of_nan_logits():
             assert torch.isfinite(loss).all() and (loss[1:] == 0).all() and (d[1:] == 0).all() and torch.isfinite(d).all()
 
 
+def test_entry_in_a_part_of_nothing_but_minus_infinity():
+    x = _x(2, 20, F32)
+    x[0, :8] = NEG
+    ids, z = torch.tensor([[3, 12], [3, 12]], device=DEV), torch.zeros(2, 2, device=DEV)
+    whole, dw = ops.distill_topk_fused(x, ids, z, 1.0)
+    st = torch.stack([ops.distill_topk_stats(x[:, a:b], ids, z, 1.0, None, a, 20) for a, b in ((0, 8), (8, 20))])
+    for a, b in ((0, 8), (8, 20)):
+        loss, d = ops.distill_topk_grad(x[:, a:b], ids, z, ops.distill_topk_join(st), 1.0, 1.0, None, a, 20)
+        oracle.close(loss, whole.cpu(), 64 * oracle.EPS * (1 + whole[1].abs().cpu()), "loss")
+        oracle.close(d, dw[:, a:b].cpu(), 64 * oracle.EPS, "dlogits")
+    assert whole[0] == float("inf")
+
+
 def test_teacher_to_student_run():
     """The operators together: a teacher's top alternatives are the student's targets, whose
     log-probabilities rise along the gradient."""
@@ -444,3 +457,14 @@ def test_no_rows():
     assert ops.token_logprobs_bwd(x, tok, st, ent, ent).shape == (0, 100)
     loss, d = ops.distill_topk_fused(x, torch.zeros(0, 3, dtype=torch.long, device=DEV), torch.zeros(0, 3, device=DEV), 1.0)
     assert loss.shape == (0,) and d.shape == (0, 100)
+
+
+def test_capture_over_a_live_graph_of_a_leaf_is_refused():
+    x, tok = _x(3, 500, F32).clone().requires_grad_(), _tok(3, 500)
+    held = ops.token_logprobs(x, tok)[0]                      # an eager graph that is still alive
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="earlier autograd graph"):
+        with torch.cuda.graph(g):
+            ops.token_logprobs(x, tok)
+    held.sum().backward()
+    assert torch.isfinite(x.grad).all()
