@@ -304,14 +304,11 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp=None, dentropy=None
     """Gradient of :func:`token_logprobs_fwd`'s logp and entropy: dlogits in the logits' type, for
     upstream gradients ``dlogp`` / ``dentropy`` (fp32 [T], None: zero).  ``out``: where to write it;
     ``out=logits`` overwrites them."""
-    if out is None:
-        out = logits.new_empty(logits.shape)
-    else:
+    if out is not None:
         torch.autograd.graph.increment_version(out)
-    if logits.is_cuda:
-        _k().token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperature, ignore_index, out)
-        return out
-    return reference.token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperature, ignore_index, out)
+    fn = _k().token_logprobs_bwd if logits.is_cuda else reference.token_logprobs_bwd
+    new = fn(logits, tokens, stats, entropy, dlogp, dentropy, temperature, ignore_index, out)
+    return new if out is None else out
 
 
 # ---------------------------------------------------------------- distillation from top logits
@@ -319,16 +316,13 @@ DISTILL_FUSED, DISTILL_STATS, DISTILL_GRAD = 0, 1, 2
 
 
 def _distill(logits, ids, z, lse, temperature, scale, rows, vocab_start, vocab_size, mode, stats, out):
-    if mode != DISTILL_STATS:
-        if out is None:
-            out = logits.new_empty(logits.shape)
-        else:
-            torch.autograd.graph.increment_version(out)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
     fn = _k().distill_topk if logits.is_cuda else reference.distill_topk
     st, sh = (scale, 0.0) if torch.is_tensor(scale) else (None, float(scale))
-    loss, part = fn(logits, ids, z, lse, temperature, st, sh, rows, vocab_start,
+    loss, part, new = fn(logits, ids, z, lse, temperature, st, sh, rows, vocab_start,
                     logits.shape[1] if vocab_size is None else vocab_size, mode, stats, out)
-    return loss, part if mode == DISTILL_STATS else out
+    return loss, part if mode == DISTILL_STATS else new if out is None else out
 
 
 def distill_topk_fused(logits, teacher_ids, teacher_logits, scale, temperature=1.0, teacher_lse=None, out=None):
@@ -466,21 +460,7 @@ def swiglu(gu):
     return _SwiGLUFn.apply(gu)
 
 
-def _refuse_live_leaf(x):
-    """A leaf's gradient accumulator belongs to the stream of the first graph that holds it.  A
-    backward pass captured on another stream while that graph lives would make the capture wait for
-    work outside it, which ends the process; the forward pass says so instead.  The accumulator lives
-    as long as a graph holds it, or what this returns."""
-    if not (x.is_cuda and x.is_leaf and x.requires_grad and torch.is_grad_enabled()):
-        return None
-    node = torch.autograd.graph.get_gradient_edge(x).node
-    stream = torch.cuda.current_stream(x.device).cuda_stream
-    if node.metadata.setdefault("kfamd_stream", stream) != stream and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("these logits are a leaf of an earlier autograd graph that is still alive: drop that "
-                           "graph's outputs before capturing, or capture the _fwd / _bwd (or fused) calls")
-    return node
-
-
+# GPU tensors go through the same two functions in C++ (ops/csrc/bindings.cpp)
 class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, temperature, top, ignore_index):
@@ -504,7 +484,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
 def token_logprobs(logits, tokens, temperature=1.0, top=0, ignore_index=-100):
     """:func:`token_logprobs_fwd` for autograd: (logp, entropy, top_ids, top_logp); the gradient runs
     through logp and entropy."""
-    held = _refuse_live_leaf(logits)      # noqa: F841 -- until the graph holds it
+    if logits.is_cuda:
+        return _k().token_logprobs_autograd(logits, tokens, temperature, top, ignore_index)
     return _TokenLogprobsFn.apply(logits, tokens, temperature, top, ignore_index)
 
 
@@ -527,5 +508,6 @@ class _DistillTopkFn(torch.autograd.Function):
 
 def distill_topk(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None):
     """:func:`distill_topk_fused`'s loss rows for autograd (the teacher gets no gradient)."""
-    held = _refuse_live_leaf(logits)      # noqa: F841 -- until the graph holds it
+    if logits.is_cuda:
+        return _k().distill_topk_autograd(logits, teacher_ids, teacher_logits, temperature, teacher_lse)
     return _DistillTopkFn.apply(logits, teacher_ids, teacher_logits, temperature, teacher_lse)

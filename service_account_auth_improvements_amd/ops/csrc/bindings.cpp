@@ -12,6 +12,9 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <hip/hip_runtime.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <map>
 #include <tuple>
@@ -339,6 +342,12 @@ void check_grad_out(const at::Tensor& x, const at::Tensor& o, const char* op) {
   }
   TORCH_CHECK(ok, op, ": out overlaps the logits without being them");
 }
+// a new tensor for the gradient, or an empty one where `out` is given and fit to take it
+at::Tensor grad_out(const at::Tensor& x, const std::optional<at::Tensor>& out, const char* op) {
+  if (!out.has_value()) return at::empty({x.size(0), x.size(1)}, x.options());
+  check_grad_out(x, *out, op);
+  return at::empty({0, 0}, x.options());
+}
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(const at::Tensor& x,
                                                                                       const at::Tensor& tokens,
@@ -367,10 +376,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log
   return {logp, entropy, stats, ids, tlp};
 }
 
-void token_logprobs_bwd(const at::Tensor& x, const at::Tensor& tokens, const at::Tensor& stats,
-                        const at::Tensor& entropy, const std::optional<at::Tensor>& dlogp,
-                        const std::optional<at::Tensor>& dentropy, double temperature, int64_t ignore_index,
-                        at::Tensor d) {
+at::Tensor token_logprobs_bwd(const at::Tensor& x, const at::Tensor& tokens, const at::Tensor& stats,
+                              const at::Tensor& entropy, const std::optional<at::Tensor>& dlogp,
+                              const std::optional<at::Tensor>& dentropy, double temperature, int64_t ignore_index,
+                              const std::optional<at::Tensor>& out) {
   const char* op = "token_logprobs_bwd";
   const int dt = check_logits(x, op);
   check_temperature(temperature, op);
@@ -380,18 +389,22 @@ void token_logprobs_bwd(const at::Tensor& x, const at::Tensor& tokens, const at:
   if (dentropy.has_value()) check_rows_f32(*dentropy, x, 0, op, "dentropy");
   c10::hip::HIPGuardMasqueradingAsCUDA g(x.device());
   const auto tok = check_tokens(tokens, x, op);
-  check_grad_out(x, d, op);
+  const at::Tensor fresh = grad_out(x, out, op);
+  const at::Tensor& d = out.has_value() ? *out : fresh;
   check_rc(kf_token_logprobs_bwd(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), x.size(0), (int)x.size(1),
                                  tok.data_ptr<int64_t>(), ignore_index, stats.data_ptr<float>(),
                                  entropy.data_ptr<float>(), dlogp.has_value() ? dlogp->data_ptr<float>() : nullptr,
                                  dentropy.has_value() ? dentropy->data_ptr<float>() : nullptr, (float)temperature,
                                  cur_stream()),
            op);
+  return fresh;
 }
 
 // mode 0: loss rows, gradient into out; 1: loss rows of an undivided vocabulary and this part's
-// statistics [T, 8]; 2: loss rows from joined statistics, gradient into out
-std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& z,
+// statistics [T, 8]; 2: loss rows from joined statistics (none with row weights: the backward pass of
+// mode 1), gradient into out.  Returns (loss rows, statistics, gradient); the gradient is empty where
+// it went to out.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& z,
                                                 const std::optional<at::Tensor>& lse, double temperature,
                                                 const std::optional<at::Tensor>& scale, double scale_h,
                                                 const std::optional<at::Tensor>& rows, int64_t vocab_start,
@@ -424,7 +437,8 @@ std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::T
   if (rows.has_value()) check_rows_f32(*rows, x, 0, op, "row weights");
   c10::hip::HIPGuardMasqueradingAsCUDA g(x.device());
   auto f32 = x.options().dtype(at::kFloat);
-  auto loss = at::empty({T}, f32);
+  const bool want_loss = !(mode == 2 && rows.has_value());
+  auto loss = at::empty({want_loss ? T : 0}, f32);
   const int64_t cols = kf_distill_stats_cols();
   const bool own_stats = mode == 1 || (mode == 0 && kf_distill_needs_stats(dt, (int)V));
   auto part = at::empty({own_stats ? T : 0, cols}, f32);
@@ -434,17 +448,110 @@ std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::T
     check_rows_f32(*stats_in, x, cols, op, "stats");
     st = stats_in->data_ptr<float>();
   }
-  TORCH_CHECK((mode == 1) != out.has_value(), op, ": out goes with a gradient");
-  if (out.has_value()) check_grad_out(x, *out, op);
-  check_rc(kf_distill_topk(x.data_ptr(), dt, x.stride(0), out.has_value() ? out->data_ptr() : nullptr,
-                           out.has_value() ? out->stride(0) : 0, T, (int)V, vocab_start, vocab_size, ids.data_ptr(),
+  TORCH_CHECK(mode != 1 || !out.has_value(), op, ": out goes with a gradient");
+  const at::Tensor fresh = mode == 1 ? at::empty({0, 0}, x.options()) : grad_out(x, out, op);
+  const at::Tensor& d = out.has_value() ? *out : fresh;
+  check_rc(kf_distill_topk(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), T, (int)V, vocab_start, vocab_size, ids.data_ptr(),
                            ids.scalar_type() == at::kInt ? 1 : 0, ids.stride(0), z.data_ptr(), zt, z.stride(0),
                            lse.has_value() ? lse->data_ptr<float>() : nullptr, (int)K, (float)temperature,
                            scale.has_value() ? scale->data_ptr<float>() : nullptr, (float)scale_h,
-                           rows.has_value() ? rows->data_ptr<float>() : nullptr, loss.data_ptr<float>(), st, (int)mode,
+                           rows.has_value() ? rows->data_ptr<float>() : nullptr,
+                           want_loss ? loss.data_ptr<float>() : nullptr, st, (int)mode,
                            cur_stream()),
            op);
-  return {loss, part};
+  return {loss, part, fresh};
+}
+
+// ---- the two for autograd, in C++: a backward pass of a small batch takes the time of its calls, and
+// half of that went into the interpreter (93 us for a distillation step of any small size)
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A leaf's gradient accumulator belongs to the stream of the first graph that holds it.  A backward
+// pass captured on another stream while that graph lives would make the capture wait for work outside
+// it, which ends the process; the forward pass says so instead.
+void refuse_live_leaf(const at::Tensor& x, const char* op) {
+  if (!at::GradMode::is_enabled() || !x.requires_grad() || !x.is_leaf()) return;
+  c10::hip::HIPGuardMasqueradingAsCUDA g(x.device());
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(cur_stream(), &cs) != hipSuccess || cs == hipStreamCaptureStatusNone) return;
+  const auto acc = torch::autograd::impl::try_get_grad_accumulator(x);
+  if (!acc) return;
+  const auto s = acc->stream();
+  TORCH_CHECK(!s.has_value() || s->id() == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().id(), op,
+              ": these logits are a leaf of an earlier autograd graph that is still alive: drop that graph's outputs before "
+              "capturing, or capture the _fwd / _bwd (or fused) calls");
+}
+
+at::Tensor upstream(const at::Tensor& g) { return g.to(at::kFloat).contiguous(); }
+std::optional<at::Tensor> maybe_upstream(const at::Tensor& g) {
+  return g.defined() ? std::optional<at::Tensor>(upstream(g)) : std::nullopt;
+}
+// differentiable once: a second derivative raises instead of being taken as zero
+at::Tensor once(const at::Tensor& d) {
+  if (!at::GradMode::is_enabled()) return d;
+  auto err = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that is differentiable once", 1);
+  return (*err)({d.detach().requires_grad_(true)})[0];
+}
+
+struct TokenLogprobsFn : torch::autograd::Function<TokenLogprobsFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& tokens, double temperature,
+                               int64_t top, int64_t ignore_index) {
+    auto [logp, entropy, stats, ids, tlp] = token_logprobs(x, tokens, temperature, top, ignore_index);
+    ctx->save_for_backward({x, tokens, stats, entropy});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->mark_non_differentiable({ids, tlp});
+    ctx->set_materialize_grads(false);
+    return {logp, entropy, ids, tlp};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    at::Tensor d;
+    if (grads[0].defined() || grads[1].defined()) {
+      const auto saved = ctx->get_saved_variables();
+      at::AutoGradMode off(false);
+      d = token_logprobs_bwd(saved[0], saved[1], saved[2], saved[3], maybe_upstream(grads[0]), maybe_upstream(grads[1]),
+                             ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt(), std::nullopt);
+    }
+    if (d.defined()) d = once(d);
+    return {d, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs_autograd(const at::Tensor& x,
+                                                                                   const at::Tensor& tokens,
+                                                                                   double temperature, int64_t top,
+                                                                                   int64_t ignore_index) {
+  refuse_live_leaf(x, "token_logprobs");
+  auto r = TokenLogprobsFn::apply(x, tokens, temperature, top, ignore_index);
+  return {r[0], r[1], r[2], r[3]};
+}
+
+struct DistillTopkFn : torch::autograd::Function<DistillTopkFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids, const at::Tensor& z,
+                            double temperature, const std::optional<at::Tensor>& lse) {
+    auto [loss, stats, none] = distill_topk(x, ids, z, lse, temperature, std::nullopt, 1.0, std::nullopt, 0, x.size(-1), 1,
+                                            std::nullopt, std::nullopt);
+    ctx->save_for_backward({x, ids, z, stats, lse.has_value() ? *lse : at::Tensor()});
+    ctx->saved_data["temperature"] = temperature;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    at::Tensor d;
+    {
+      at::AutoGradMode off(false);
+      const auto lse = saved[4].defined() ? std::optional<at::Tensor>(saved[4]) : std::nullopt;
+      d = std::get<2>(distill_topk(saved[0], saved[1], saved[2], lse, ctx->saved_data["temperature"].toDouble(),
+                                   std::nullopt, 1.0, upstream(grads[0]), 0, saved[0].size(1), 2, saved[3], std::nullopt));
+    }
+    return {once(d), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+at::Tensor distill_topk_autograd(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& z, double temperature,
+                                 const std::optional<at::Tensor>& lse) {
+  refuse_live_leaf(x, "distill_topk");
+  return DistillTopkFn::apply(x, ids, z, temperature, lse);
 }
 
 // ---------------- Flash attention (K3) ----------------
@@ -998,10 +1105,14 @@ TORCH_LIBRARY(kfamd, m) {
   m.def("token_logprobs(Tensor logits, Tensor tokens, float temperature, int top, int ignore_index) -> "
         "(Tensor, Tensor, Tensor, Tensor, Tensor)", &token_logprobs);
   m.def("token_logprobs_bwd(Tensor logits, Tensor tokens, Tensor stats, Tensor entropy, Tensor? dlogp, Tensor? dentropy, "
-        "float temperature, int ignore_index, Tensor(a!) out) -> ()", &token_logprobs_bwd);
+        "float temperature, int ignore_index, Tensor(a!)? out) -> Tensor", &token_logprobs_bwd);
   m.def("distill_topk(Tensor logits, Tensor ids, Tensor z, Tensor? lse, float temperature, Tensor? scale, float scale_h, "
-        "Tensor? rows, int vocab_start, int vocab_size, int mode, Tensor? stats, Tensor(a!)? out) -> (Tensor, Tensor)",
+        "Tensor? rows, int vocab_start, int vocab_size, int mode, Tensor? stats, Tensor(a!)? out) -> (Tensor, Tensor, Tensor)",
         &distill_topk);
+  m.def("token_logprobs_autograd(Tensor logits, Tensor tokens, float temperature, int top, int ignore_index) -> "
+        "(Tensor, Tensor, Tensor, Tensor)", &token_logprobs_autograd);
+  m.def("distill_topk_autograd(Tensor logits, Tensor ids, Tensor z, float temperature, Tensor? lse) -> Tensor",
+        &distill_topk_autograd);
   m.def("flash_fwd", &flash_fwd);
   m.def("flash_bwd", &flash_bwd);
   m.def("decode_attn", &decode_attn);

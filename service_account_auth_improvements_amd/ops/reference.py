@@ -160,6 +160,8 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperat
     for t, name in ((dlogp, "dlogp"), (dentropy, "dentropy")):
         if t is not None:
             _check_rows(t, logits, (), op, name)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype)
     _check_out(out, logits, op)
     V = logits.shape[1]
     z = torch.zeros(logits.shape[0], 1)
@@ -177,7 +179,7 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperat
 
 def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_start, vocab_size, mode, stats, out):
     """ops.distill_topk_*: mode 0 loss rows and gradient; 1 loss rows and statistics [T, 8]; 2 loss rows
-    and gradient from joined statistics.  Returns (loss, statistics)."""
+    and gradient from joined statistics.  Returns (loss, statistics, gradient)."""
     op = "distill_topk"
     _check_logits(logits, temperature, op)
     T, V = logits.shape
@@ -201,8 +203,10 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
         _check_rows(rows, logits, (), op, "row weights")
     if mode == 2:
         _check_rows(stats, logits, (8,), op, "stats")
-    if out is not None:
-        _check_out(out, logits, op)
+    _need(mode != 1 or out is None, f"{op}: out goes with a gradient")
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype)
+    _check_out(out, logits, op)
     nan, zero = float("nan"), torch.zeros(())
     ids = ids.long()
     has = ids >= 0
@@ -250,13 +254,13 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
     loss = loss + torch.where(live, r1 * (torch.log(r1) - (torch.log(u) - logs)), zero).squeeze(1)
     loss = loss.masked_fill(~some, 0.0).masked_fill(bad, nan)
     if mode == 1:
-        return loss, part.masked_fill(~some.unsqueeze(1), 0.0).masked_fill(bad.unsqueeze(1), nan)
+        return loss, part.masked_fill(~some.unsqueeze(1), 0.0).masked_fill(bad.unsqueeze(1), nan), None
     p = torch.exp((x - m) / temperature - logs)
     dx = torch.where(inside, p * W, p * torch.where(live, W - r1 * s / u, W))
     dx = torch.cat([dx, torch.zeros(T, 1)], 1).scatter_add_(1, col, torch.where(here, -q, zero))[:, :V]
     dx = dx * (scale_h / temperature) * (1.0 if rows is None else rows.unsqueeze(1))
     out.copy_(dx.masked_fill(~some.unsqueeze(1), 0.0).masked_fill(bad.unsqueeze(1), nan))
-    return loss, None
+    return loss, None, out
 
 
 def adamw_(p, w, m, v, g, n_decay, lr, b1, b2, eps, wd, step, gscale=1.0, sumsq=None,

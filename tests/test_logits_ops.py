@@ -207,20 +207,3 @@ def refusal_args(device):
 def test_refusals(what):
     with pytest.raises(RuntimeError, match="token_logprobs|distill_topk"):
         REFUSALS[what](refusal_args("cpu"))
-
-
-def test_capture_over_a_live_graph_of_a_leaf_is_refused(monkeypatch):
-    class Leaf:
-        is_cuda, is_leaf, requires_grad, device = True, True, True, "cuda:0"
-    real = torch.zeros(2, 3, requires_grad=True)
-    held = real.sum()                      # an eager graph that keeps the leaf's accumulator alive
-    streams = iter([type("S", (), {"cuda_stream": 1}), type("S", (), {"cuda_stream": 2}), type("S", (), {"cuda_stream": 1})])
-    edge = torch.autograd.graph.get_gradient_edge(real)
-    monkeypatch.setattr(torch.autograd.graph, "get_gradient_edge", lambda _: edge)
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda _d: next(streams))
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
-    ops._refuse_live_leaf(Leaf())          # first graph: stream 1
-    with pytest.raises(RuntimeError, match="leaf of an earlier autograd graph"):
-        ops._refuse_live_leaf(Leaf())      # capture on stream 2
-    ops._refuse_live_leaf(Leaf())          # the leaf's own stream
-    assert held.requires_grad

@@ -459,12 +459,50 @@ def test_no_rows():
     assert loss.shape == (0,) and d.shape == (0, 100)
 
 
-def test_capture_over_a_live_graph_of_a_leaf_is_refused():
+@pytest.mark.parametrize("other", [False, True])
+def test_capture_over_a_live_graph_of_a_leaf_is_refused(other):
     x, tok = _x(3, 500, F32).clone().requires_grad_(), _tok(3, 500)
-    held = ops.token_logprobs(x, tok)[0]                      # an eager graph that is still alive
-    g = torch.cuda.CUDAGraph()
-    with pytest.raises(RuntimeError, match="earlier autograd graph"):
-        with torch.cuda.graph(g):
-            ops.token_logprobs(x, tok)
+    ids, z = torch.zeros(3, 2, dtype=torch.long, device=DEV), torch.zeros(3, 2, device=DEV)
+    held = (x * 2) if other else ops.token_logprobs(x, tok)[0]      # an eager graph that is still alive
+    for call in (lambda: ops.token_logprobs(x, tok), lambda: ops.distill_topk(x, ids, z)):
+        with pytest.raises(RuntimeError, match="earlier autograd graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
     held.sum().backward()
     assert torch.isfinite(x.grad).all()
+
+
+def test_autograd_corners():
+    x, tok = _x(4, 300, F32).clone().requires_grad_(), _tok(4, 300)
+    ids, z, L = (t.to(DEV) for t in _teacher(4, 300, 5, F32, True, 1.0))
+    # one output used, or none
+    logp, ent, top, tlp = ops.token_logprobs(x, tok, 1.0, 3)
+    assert not top.requires_grad and not tlp.requires_grad
+    (d,) = torch.autograd.grad(ent.sum(), x)
+    ref, size = oracle.logprobs_grad(x.detach().cpu(), tok.cpu(), torch.zeros(4), torch.ones(4))
+    oracle.close(d, ref, oracle.grad_bound(ref, size, 60.0, 300, F32), "entropy's")
+    # 16-bit upstream gradients, no gradient wanted, leaf of another type
+    xh = x.detach().half().requires_grad_()
+    loss = ops.distill_topk(xh, ids, z, 1.0, L)
+    loss.to(torch.bfloat16).sum().backward()
+    assert xh.grad.dtype == FP16
+    with torch.no_grad():
+        assert not ops.distill_topk(x, ids, z).requires_grad
+    assert not ops.token_logprobs(x.detach(), tok)[0].requires_grad
+    # differentiable once
+    for f in (lambda: ops.token_logprobs(x, tok)[0].sum(), lambda: ops.distill_topk(x, ids, z).pow(2).sum()):
+        (g,) = torch.autograd.grad(f(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            g.sum().backward()
+    # logits overwritten before the backward pass
+    y = x * 1.0
+    lo = ops.distill_topk(y, ids, z)
+    with torch.no_grad():
+        y.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lo.sum().backward()
+    # refusals come through
+    with pytest.raises(RuntimeError, match="distill_topk"):
+        ops.distill_topk(x, ids.short(), z)
+    with pytest.raises(RuntimeError, match="token_logprobs"):
+        ops.token_logprobs(x, tok.int())
