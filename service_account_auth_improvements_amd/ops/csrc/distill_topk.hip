@@ -102,6 +102,8 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(const void* logits
     const bool more = rn < T;
     const char* rown = row_at(more ? rn : r);
     char* orow = (char*)out + r * ldo * Elem<DT>::bytes;
+    // the thread that holds an element: that of its piece, or of its place in the tail
+    auto owner = [&](int c) { return c < N * nfull ? (c / N) % NT : c - N * nfull; };
     // ---- the teacher's row: thread k holds entry k
     head[tid] = 0;
     const bool mine = id >= 0 && id < V;
@@ -128,21 +130,23 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(const void* logits
         if (n != n) W = n;                               // a NaN entry: the whole row
       }
       if (tid < K) { sid[tid] = mine ? id : -1; sq[tid] = q; slq[tid] = lq; sx[tid] = x; }
-      if (mine) {
-        // the thread that holds the element: that of its piece, or of its place in the tail
-        const int own = id < N * nfull ? (id / N) % NT : id - N * nfull;
-        next[tid] = atomicExch(&head[own], tid + 1);
-      }
+      if (mine) next[tid] = atomicExch(&head[owner(id)], tid + 1);
     }
     lds_barrier();
     bool first = mine;                                   // of the entries with this id
     if (mine) {
-      float qs = 0.f;                                    // the same id twice: its entries add up, in order
-#pragma unroll 4
-      for (int k = 0; k < K; ++k) {
-        const bool same = sid[k] == id;
-        qs += same ? sq[k] : 0.f;
-        first = first && !(same && k < tid);
+      // the same id twice: its entries add up.  They are in one list; its order is that of the
+      // atomics, so the sum is formed in the order of the entries
+      bool twice = false;
+      for (int h = head[owner(id)]; h; h = next[h - 1]) {
+        const bool same = h - 1 != tid && sid[h - 1] == id;
+        twice = twice || same;
+        first = first && !(same && h - 1 < tid);
+      }
+      float qs = sq[tid];
+      if (twice) {
+        qs = 0.f;
+        for (int k = 0; k < K; ++k) qs += sid[k] == id ? sq[k] : 0.f;
       }
       sqs[tid] = qs;
     }
@@ -163,9 +167,11 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(const void* logits
           const u32 kept = DT == DT_FP32 ? 0u : (c & 1) ? 0xffffu : 0xffff0000u;
           const u32 fill = Elem<DT>::neg_inf & ~kept;
 #pragma unroll
-          for (int j = 0; j < RES; ++j)
+          for (int j = 0; j < RES; ++j) {
+            if (__ballot(at >> 2 == j) == 0) continue;       // no thread of the wave has one in this piece
 #pragma unroll
             for (int w = 0; w < 4; ++w) b[j][w] = at == 4 * j + w ? (b[j][w] & kept) | fill : b[j][w];
+          }
         }
       }
     }
@@ -448,14 +454,21 @@ __global__ __launch_bounds__(GRAD_NT) void distill_grad_kernel(const void* logit
     sx[at] = x;
   }
   lds_barrier();
+  // the thread that holds an element: that of its piece, or of its place in the tail
+  auto owner = [&](int c) { return c < N * nfull ? (c / N - p0) % GRAD_NT : c - N * nfull; };
+  if (tid < nin) next[tid] = atomicExch(&head[owner(scol[tid])], tid + 1);
+  lds_barrier();
   if (tid < nin) {
+    // the same id twice: as in the fused kernel
     const int c = scol[tid];
-    float qs = 0.f;                      // the same id twice: its entries add up, in order
-    for (int k = 0; k < nin; ++k) qs += scol[k] == c ? sq[k] : 0.f;
+    bool twice = false;
+    for (int h = head[owner(c)]; h; h = next[h - 1]) twice = twice || (h - 1 != tid && scol[h - 1] == c);
+    float qs = sq[tid];
+    if (twice) {
+      qs = 0.f;
+      for (int k = 0; k < nin; ++k) qs += scol[k] == c ? sq[k] : 0.f;
+    }
     sqs[tid] = qs;
-    // the thread that holds the element: that of its piece, or of its place in the tail
-    const int own = c < N * nfull ? (c / N - p0) % GRAD_NT : c - N * nfull;
-    next[tid] = atomicExch(&head[own], tid + 1);
   }
   lds_barrier();
   const bool use_rest = REST && rest > 0.f && !(u == 0.f);
