@@ -56,7 +56,8 @@ struct Teacher {
 // loads of one row and the stores of another are in flight while the exponentials are computed.
 // 4096 rows of 128256 bf16 logits: 415-440 us (5.1 TB/s; a copy of the same bytes takes 430), where
 // two passes over rows, the second from the caches, take 525 and a block per row without the
-// reads ahead takes 600.
+// reads ahead takes 600.  Groups of pieces behind a row's end are jumped over by the whole block:
+// 4096 rows of 4000 bf16 logits take 25 us, and 70 where every thread goes through all sixteen.
 constexpr int RES = 16;              // pieces of a thread
 constexpr int GRP = 2;               // pieces summed together
 
@@ -180,6 +181,7 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(const void* logits
     RowStat st = stat_empty();
 #pragma unroll
     for (int g = 0; g < RES; g += GRP) {
+      if (g * NT >= nfull) continue;                     // behind the end for the whole block
       float f[GRP][N];
       float bm = st.m;
 #pragma unroll
@@ -231,6 +233,7 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(const void* logits
     }
 #pragma unroll
     for (int j = 0; j < RES; ++j) {
+      if (j * NT >= nfull) continue;
       float f[N];
       unpack_piece<DT>(b[j], f);
 #pragma unroll
