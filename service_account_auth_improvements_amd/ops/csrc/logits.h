@@ -150,6 +150,19 @@ __device__ __forceinline__ float wave_reduce(float v, float neutral, Op op) {
   v = dpp_step<0x143, 0xc>(v, neutral, op);      // row_bcast:31 into rows 2 and 3
   return lane_value(v, 63);
 }
+__device__ __forceinline__ u32 wave_max(u32 v) {           // 0 is neutral
+  const auto step = [&](auto ctrl, auto rows) {
+    v = max(v, (u32)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return (u32)__builtin_amdgcn_readlane((int)v, 63);
+}
 // `red` holds NT / 64 values and is not written again before another barrier
 template <int NT, typename Op>
 __device__ __forceinline__ float block_reduce(float v, float neutral, float* red, Op op, int tid) {

@@ -50,13 +50,8 @@ __device__ __forceinline__ u32 wave_kth(const u32* key, int k) {
     hi = max(hi, v[i]);
     lo = min(lo, v[i]);
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    hi = max(hi, (u32)__shfl_xor((int)hi, o, 64));
-    lo = min(lo, (u32)__shfl_xor((int)lo, o, 64));
-  }
-  hi = __builtin_amdgcn_readfirstlane(hi);
-  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = wave_max(hi);
+  lo = ~wave_max(~lo);
   if (hi == lo) return lo;
   u32 bit = 0x80000000u >> __clz(hi ^ lo);
   u32 t = hi & ~(2 * bit - 1);                   // the bits that all keys share
@@ -74,9 +69,9 @@ __device__ __forceinline__ u32 wave_kth(const u32* key, int k) {
   return t;
 }
 
-// out(rank, key) for the keys of rank < k among the n (<= 1024) different keys at `key`, by all threads
-// of a block of nt: `per` neighbouring threads (a power of two) count a share of the others each.
-// The list is 16-byte aligned and filled up with zeros to a multiple of 4.
+// out(rank, key) for the keys of rank < k among the n different keys at `key`, by all threads of a
+// block of nt: `per` neighbouring threads (a power of two) count a share of the others each.  n^2
+// comparisons: for some hundred keys.  The list is 16-byte aligned and filled up with zeros to a multiple of 4.
 typedef __attribute__((ext_vector_type(2))) u64 u64x2;
 template <typename Out>
 __device__ __forceinline__ void block_rank(const u64* key, int n, int k, int tid, int nt, Out out) {
@@ -294,8 +289,9 @@ __global__ __launch_bounds__(NT, 8) void logprobs_kernel(const void* __restrict_
   }
 }
 
-// Few rows: one CU alone takes 8.8 us for the exponentials of 128256 logits, so a row goes to
-// `parts` blocks of PART_NT threads and a second launch joins their statistics and alternatives.
+// Few long rows: one CU alone takes 8 us to read 128256 bf16 logits and form their exponentials, so a
+// row goes to `parts` blocks of PART_NT threads and a second launch joins their statistics and
+// alternatives.
 constexpr int PART_NT = 256;
 struct Part {
   RowStat st;
@@ -325,7 +321,11 @@ __global__ __launch_bounds__(PART_NT, 8) void logprobs_part_kernel(const void* _
   }
 }
 
-constexpr int JOIN_NT = 1024, JOIN_KEYS = 1024, PARTS_MAX = 16;
+// The parts' alternatives are `parts` lists of k keys in order.  The first ones of each list, 256
+// together, give a bound as the groups' maxima above, and some k + 16 keys reach it: those are
+// ranked.  Up to 192 keys are ranked as they are, which takes less than finding the bound (160 keys:
+// 13.3 us a call against 13.6; 320: 12.2 against 9.6, 1024: 32 against 10.5).
+constexpr int JOIN_NT = 512, PARTS_MAX = 16, JOIN_KEYS = PARTS_MAX * TOP_MAX, JOIN_DIRECT = 192;
 
 template <int DT>
 __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const void* __restrict__ logits, long ld, int V,
@@ -333,23 +333,48 @@ __global__ __launch_bounds__(JOIN_NT) void logprobs_join_kernel(const void* __re
                                                                 float inv_temp, int k, int parts,
                                                                 const Part* __restrict__ part,
                                                                 const u64* __restrict__ keys, Result o) {
-  __shared__ alignas(16) u64 key[JOIN_KEYS + 4];
+  constexpr int HELD = JOIN_KEYS / JOIN_NT;
+  __shared__ alignas(16) u64 cand[JOIN_KEYS + 4];
+  __shared__ u32 first[GROUPS], bound;
+  __shared__ int ncand;
   const long r = blockIdx.x;
   const int tid = threadIdx.x, n = parts * k;
   const long t = tokens[r];
-  const bool in = t >= 0 && t < V;
+  const bool in = t >= 0 && t < V, direct = n <= JOIN_DIRECT;
   const float x = in ? load1<DT>((const char*)logits + r * ld * Elem<DT>::bytes, t) : 0.f;
   const int l = tid & 15;
   const RowStat mine = l < parts ? part[r * parts + l].st : stat_empty();
-  for (int i = tid; i < n; i += blockDim.x) key[i] = keys[r * n + i];
-  if (tid < 4) key[n + tid] = 0;
+  u64 key[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) key[i] = tid + i * JOIN_NT < n ? keys[r * n + tid + i * JOIN_NT] : 0;
+  if (!direct && tid < GROUPS) {
+    // parts >= 2; `each` a power of two: with fewer than k keys in `first` the bound would be 0
+    const int each = GROUPS >> (32 - __clz(parts - 1)), q = tid / each, at = tid & (each - 1);
+    first[tid] = q < parts && at < k ? (u32)(keys[r * n + q * k + at] >> 32) : 0u;
+  }
   if (t == ignore) return write_ignored(o, r, k, tid, blockDim.x);
   const RowStat st = lanes_stat<MOMENT, 16>(mine, a);
   const float L = __log2f(st.s);
   if (tid == 0) write_row(o, r, st, L, in, x, inv_temp);
   if (k == 0) return;
+  for (int i = tid; i < n + 4; i += JOIN_NT) cand[i] = 0;
+  if (tid == 0) {
+    ncand = 0;
+    bound = 1;                                   // key 0: a part of fewer than k logits
+  }
   __syncthreads();
-  block_rank(key, n, k, tid, blockDim.x, [&](int rank, u64 v) { write_top(o, r, k, rank, v, st.m, L, inv_temp); });
+  if (!direct) {
+    if (tid < 64) {
+      const u32 b = wave_kth(first, k);
+      if (tid == 0) bound = max(b, 1u);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+    if ((u32)(key[i] >> 32) >= bound) cand[atomicAdd(&ncand, 1)] = key[i];
+  __syncthreads();
+  block_rank(cand, ncand, k, tid, JOIN_NT, [&](int rank, u64 v) { write_top(o, r, k, rank, v, st.m, L, inv_temp); });
 }
 
 // gradient: one block per 4 pieces a thread of a row, nothing to reduce
@@ -407,13 +432,15 @@ __global__ __launch_bounds__(BWD_NT) void logprobs_bwd_kernel(const void* logits
   }
 }
 
-// Blocks of one row for `rows` rows of np pieces: 1 from 256 rows on, where a block per row fills
-// the 256 CUs; below that up to two blocks a CU, with at least two pieces a thread, as many as the
-// join holds.
+// Blocks of one row for `rows` rows of np pieces.  A row is split where one block would take longer
+// than two launches: from 8192 pieces on with alternatives, whose ranking the parts do twice, and
+// from 4096 without (24 rows of 50021 bf16 logits: 5.9 us split and 7.0 whole without alternatives,
+// 12.0 and 11.1 with 20; of 32000 5.4 whole, 4.9 split and 8.9, 10.3; of 128256 5.6, 10.9 and 11.1,
+// 15.5), and below 128 rows, where the two take the same (128256 logits: 11.9 and 12.1 us).  Then up to
+// two blocks a CU, with at least two pieces a thread.
 static int split_parts(long rows, int np, int k) {
-  long p = std::min<long>(512 / std::max<long>(rows, 1), cdiv(np, 2 * PART_NT));
-  p = std::min<long>(p, std::min(PARTS_MAX, k > 0 ? JOIN_KEYS / k : PARTS_MAX));
-  return rows >= 256 || p < 2 ? 1 : (int)p;
+  if (rows >= 128 || np <= (k > 0 ? 8192 : 4096)) return 1;
+  return (int)std::min<long>(std::min<long>(512 / std::max<long>(rows, 1), cdiv(np, 2 * PART_NT)), PARTS_MAX);
 }
 
 }  // namespace
@@ -438,7 +465,7 @@ int kf_token_logprobs(const void* logits, int dt, long ld, long rows, int V, con
     constexpr int DT = decltype(DTc)::value;
     const int np = (V + Elem<DT>::N - 1) / Elem<DT>::N, parts = split_parts(rows, np, k);
     if (parts > 1) {
-      const int per = cdiv(cdiv(np, parts), PART_NT) * PART_NT;
+      const int per = cdiv(cdiv(np, parts), 64) * 64;           // the lanes of a wave end together
       const Result o{logp, entropy, stats, top, ids};
       Part* part = (Part*)scratch;
       u64* keys = (u64*)(part + rows * parts);
@@ -463,9 +490,12 @@ int kf_token_logprobs(const void* logits, int dt, long ld, long rows, int V, con
       // eight to sixteen pieces a thread: 4000 rows of 128256 bf16 logits take 157 us with 1024
       // threads and 172 with 512, of 32000 logits 52 and 47.  With alternatives smaller blocks: more
       // of them share a CU, and some read while others rank (2500 rows of 128256: 131 us with 1024,
-      // 124 with 512; 4000 rows of 32000: 95 with 1024, 66 with 512, 62 with 256)
+      // 124 with 512; 4000 rows of 32000: 95 with 1024, 66 with 512, 62 with 256).  Up to 512 rows
+      // are held at once also as blocks of 1024 threads (256 rows of 50021, 20 alternatives: 12.8 us
+      // with 1024, 15.2 with 256; 512 rows of 128256: 32.1 and 32.3 with 512; 700: 43.8 and 41.8)
       if (k > 0) {
-        if (np > 8192) go(std::integral_constant<int, 512>{}, std::true_type{});
+        if (np > 4096 && rows <= 512) go(std::integral_constant<int, 1024>{}, std::true_type{});
+        else if (np > 8192 || (np > 2048 && rows <= 512)) go(std::integral_constant<int, 512>{}, std::true_type{});
         else go(std::integral_constant<int, 256>{}, std::true_type{});
       } else {
         if (np > 8192) go(std::integral_constant<int, 1024>{}, std::false_type{});

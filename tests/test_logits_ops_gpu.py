@@ -145,6 +145,39 @@ def test_few_and_many_rows(T):
         _check_fwd(x, tok, 0.9, top)
 
 
+@pytest.mark.parametrize("V,dtype", [(70001, BF16), (66003, FP16), (36001, F32)])
+def test_few_long_rows_with_masks_ties_and_orders(V, dtype):
+    """Rows that several blocks share: their lists of alternatives meet in one order, whatever is equal."""
+    low = torch.finfo(dtype).min
+    x, tok = _x(13, V, dtype, 4, 1), _tok(13, V)
+    ar = torch.arange(V, device=DEV)
+    x[0] = NEG; x[0, int(tok[0])] = 2.0
+    x[1] = 1.5                                              # all equal
+    x[2] = low
+    x[3].masked_fill_(ar % 5 != 0, low)
+    x[4, 700:] = NEG                                        # one part holds all there is
+    x[5, :V - 9] = NEG                                      # ... the last one
+    x[6] = torch.sort(x[6].float(), descending=True).values.to(dtype)
+    x[7] = torch.sort(x[7].float()).values.to(dtype)
+    x[8] = (x[8].float() / 4).round().to(dtype)             # some ten values in all
+    x[9, V // 2] = float("nan")
+    x[10] = NEG; x[10, 1::V // 40] = 3.0
+    x[11] = float("nan")
+    x[12] = NEG; tok[12] = -100
+    for top in (0, 1, 5, 12, 13, 20, 64, 128):              # up to and above what is ranked directly
+        _check_fwd(x, tok, 1.3, top)
+
+
+@pytest.mark.parametrize("T", [2, 33, 70, 127, 128, 512, 513])
+@pytest.mark.parametrize("V,top", [(32769, 0), (36800, 20), (65537, 64), (65537, 128), (140001, 33)])
+def test_rows_around_the_choices_of_the_launch(T, V, top):
+    if T * V > 20_000_000:
+        V = V // 2 + 1
+    x, tok = _x(T, V, BF16, 5, 3), _tok(T, V)
+    tok[T // 2] = -100
+    _check_fwd(x, tok, 0.8, top)
+
+
 def test_logprobs_expanded_and_broadcast_inputs():
     x = _x(1, 3001, BF16).expand(7, 3001)                    # row stride 0
     tok = _tok(7, 3001)
