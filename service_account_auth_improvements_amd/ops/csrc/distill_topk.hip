@@ -216,6 +216,7 @@ __global__ __launch_bounds__(NT, 4) void distill_fused_kernel(const void* logits
     }
 #pragma unroll
     for (int j = 0; j < RES; ++j) asm volatile("" : "+v"(b[j]));        // unpacked anew below, not kept
+    asm volatile("" : "+s"(nfull));                      // nor are the comparisons with it
     st = block_stat<REST ? SUBSET : PLAIN, NT>(st, a, red3, tid);
     const float m = st.m, s = st.s, u = st.u;
     const float L = __log2f(s);
@@ -302,8 +303,7 @@ __device__ __forceinline__ RowStat walk_sums(const char* row, int V, float a, co
   };
   for (int c = threadIdx.x; c < nfull; c += UN * NT) {
     u32x4 v[UN];
-#pragma unroll
-    for (int j = 0; j < UN; ++j) v[j] = load_piece<DT>(row, min(c + j * NT, nfull - 1));
+    load_pieces<DT>(row, [&](int j) { return min(c + j * NT, nfull - 1); }, v);
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
       unpack_piece<DT>(v[j], f[j]);

@@ -211,8 +211,7 @@ __device__ __forceinline__ RowStat walk_row(const char* row, int V, int p0, int 
   int c = p0 + threadIdx.x;
   for (; c + (UN - 1) * NT < nfull; c += UN * NT) {
     u32x4 r[UN];
-#pragma unroll
-    for (int j = 0; j < UN; ++j) r[j] = load_piece<DT>(row, c + j * NT);
+    load_pieces<DT>(row, [&](int j) { return c + j * NT; }, r);
 #pragma unroll
     for (int j = 0; j < UN; ++j) unpack_piece<DT>(r[j], f[j]);
     eat(c, UN);
@@ -220,8 +219,7 @@ __device__ __forceinline__ RowStat walk_row(const char* row, int V, int p0, int 
   if (c < nfull) {
     // the rest, loaded together: pieces behind the end are the last full one again, read as -inf
     u32x4 r[UN];
-#pragma unroll
-    for (int j = 0; j < UN; ++j) r[j] = load_piece<DT>(row, min(c + j * NT, nfull - 1));
+    load_pieces<DT>(row, [&](int j) { return min(c + j * NT, nfull - 1); }, r);
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
       unpack_piece<DT>(r[j], f[j]);

@@ -267,6 +267,35 @@ def test_distill(T, V, pad, skip, K, dtype, zt, lse):
     assert d2.data_ptr() == x.data_ptr() and torch.equal(lo2, loss) and torch.equal(x, d)
 
 
+# every row (skip odd, stride even) or every second one
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("V,pad,skip", [(1, 0, 1), (2, 1, 0), (8, 1, 0), (9, 0, 0), (16, 1, 1), (17, 1, 1), (520, 3, 0), (4096, 1, 0), (32769, 0, 0),
+                                        (66000, 1, 0), (131072, 1, 1), (131080, 1, 0)])
+def test_rows_off_a_4_byte_boundary(V, pad, skip, dtype):
+    T, k = 6, min(V, 7)
+    x, tok = _x(T, V, dtype, 6, pad, skip), _tok(T, V)
+    x[0, 0] = x[1, 0] = 30.0                                 # the first element is the greatest
+    x[2] = 0.25                                              # equal everywhere: the first ones
+    x[3, 0] = NEG
+    x[4, 1:] = NEG; x[4, 0] = -5.0                           # there is no other
+    tok[0] = tok[1] = tok[4] = 0
+    ent, stats = _check_fwd(x, tok, 1.2, k)
+    _check_fwd(x[:, V // 2:], tok % (V - V // 2), 1.2, 0)
+    # the same bits wherever a row lies
+    there = torch.zeros(T, V + 16 - V % 8, dtype=dtype, device=DEV)[:, :V]
+    there.copy_(x)
+    for a, b in zip(ops.token_logprobs_fwd(x, tok, 1.2, k), ops.token_logprobs_fwd(there, tok, 1.2, k)):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a[~a.isnan()], b[~b.isnan()])    # V = 1 has a row of -inf
+    ids = torch.stack([(torch.arange(k) * max(1, V // k) + r % 2) % V for r in range(T)])
+    ids[5] = 0                                               # the first element again and again
+    z = torch.linspace(2, -2, k).expand(T, k).clone()
+    for L in (None, torch.logsumexp(z, 1) + 0.2):
+        _check_kd(x, ids, z, 1.0, L)
+    want = ops.distill_topk_fused(x, ids.to(DEV), z.to(DEV), 1.0, 1.0)[1]
+    here = ops.distill_topk_fused(x, ids.to(DEV), z.to(DEV), 1.0, 1.0, out=x)[1]
+    assert torch.equal(here.contiguous().view(torch.int16), want.view(torch.int16))      # bits: V = 1 has a row of -inf, all NaN
+
+
 @pytest.mark.parametrize("V", [400, 20000])
 @pytest.mark.parametrize("lse", [False, True])
 def test_distill_masks_and_special_rows(V, lse):
