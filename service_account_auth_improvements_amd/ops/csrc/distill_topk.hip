@@ -58,7 +58,9 @@ struct Teacher {
 // two passes over rows, the second from the caches, take 525 and a block per row without the
 // reads ahead takes 600.  Groups of pieces behind a row's end are jumped over by the whole block:
 // 4096 rows of 4000 bf16 logits take 25 us, and 70 where every thread goes through all sixteen.
-constexpr int RES = 16;              // pieces of a thread
+// Rows that four pieces a thread of the smallest block hold leave registers for half as many
+// blocks more on a CU: 20 us.
+constexpr int RES_MAX = 16, RES_SHORT = 4;       // pieces of a thread
 constexpr int GRP = 2;               // pieces summed together
 
 // piece j of thread t; behind the last full piece: some full piece
@@ -70,11 +72,14 @@ __device__ __forceinline__ u32x4 load_mine(const char* row, int j, int nfull, in
   return *(const u32x4_a2*)(base + (size_t)(u32)(min(t, last) * 16));
 }
 
-// 128 registers a thread: 16 waves fill a CU
-template <int DT, int NT, bool REST>
-__global__ __launch_bounds__(NT, 4) void distill_fused_kernel(const void* logits, long ld, void* out, long ldo, long T,
-                                                              int V, Teacher te, float temp, const float* scale_ptr,
-                                                              float scale_h, float* loss, int keep) {
+// 128 registers a thread: 16 waves fill a CU; of rows of RES_SHORT 24 (32 would be as fast, with
+// scalar registers spilled)
+constexpr int fused_waves(int res) { return res == RES_SHORT ? 6 : 4; }
+
+template <int DT, int NT, int RES, bool REST>
+__global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
+    const void* logits, long ld, void* out, long ldo, long T, int V, Teacher te, float temp, const float* scale_ptr,
+    float scale_h, float* loss, int keep) {
   constexpr int N = Elem<DT>::N;
   __shared__ float red[5][NT / 64];
   __shared__ RowStat red3[NT / 64];
@@ -507,7 +512,7 @@ int cu_count() {
 
 bool fits_registers(int dt, int V) {
   const int n = dt == DT_FP32 ? 4 : 8;
-  return V >= n && V / n <= 1024 * RES;
+  return V >= n && V / n <= 1024 * RES_MAX;
 }
 
 // outputs of more than the last-level cache's 256 MB leave nothing in it for their reader: they are
@@ -540,21 +545,24 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
     const long bytes = (long)V * (dt == DT_FP32 ? 4 : 2);
     const int keep = rows * bytes <= CACHE_BYTES;
     by_type(dt, [&](auto DTc) {
-      auto go = [&](auto NTc, auto Rc) {
-        constexpr int DT = decltype(DTc)::value, NT = decltype(NTc)::value;
-        const unsigned grid = (unsigned)std::min<long>(rows, (long)cu_count() * (1024 / NT));
-        distill_fused_kernel<DT, NT, decltype(Rc)::value><<<grid, NT, 0, s>>>(logits, ld, out, ldo, rows, V, te, temp,
-                                                                             scale_ptr, scale_h, loss, keep);
+      auto go = [&](auto NTc, auto Sc, auto Rc) {
+        constexpr int DT = decltype(DTc)::value, NT = decltype(NTc)::value, RES = decltype(Sc)::value;
+        const unsigned grid = (unsigned)std::min<long>(rows, (long)cu_count() * (256 * fused_waves(RES) / NT));
+        distill_fused_kernel<DT, NT, RES, decltype(Rc)::value><<<grid, NT, 0, s>>>(
+            logits, ld, out, ldo, rows, V, te, temp, scale_ptr, scale_h, loss, keep);
       };
-      auto by_rest = [&](auto NTc) {
-        if (lse) go(NTc, std::true_type{});
-        else go(NTc, std::false_type{});
+      auto by_rest = [&](auto NTc, auto Sc) {
+        if (lse) go(NTc, Sc, std::true_type{});
+        else go(NTc, Sc, std::false_type{});
       };
       // the smallest block that holds a row: more of them share a CU
       const int np = V / Elem<decltype(DTc)::value>::N;
-      if (np <= 256 * RES) by_rest(std::integral_constant<int, 256>{});
-      else if (np <= 512 * RES) by_rest(std::integral_constant<int, 512>{});
-      else by_rest(std::integral_constant<int, 1024>{});
+      using Short = std::integral_constant<int, RES_SHORT>;
+      using Long = std::integral_constant<int, RES_MAX>;
+      if (np <= 256 * RES_SHORT) by_rest(std::integral_constant<int, 256>{}, Short{});
+      else if (np <= 256 * RES_MAX) by_rest(std::integral_constant<int, 256>{}, Long{});
+      else if (np <= 512 * RES_MAX) by_rest(std::integral_constant<int, 512>{}, Long{});
+      else by_rest(std::integral_constant<int, 1024>{}, Long{});
     });
     return 0;
   }

@@ -260,7 +260,7 @@ __device__ __forceinline__ void write_top(const Result& o, long r, int k, int ra
 }
 
 // one block per row; 8 waves a SIMD (registers of both kinds: 100 scalar ones already halve that), so
-// that blocks share a CU and some read while others rank: 2048 rows with 64 alternatives 111 us, 143
+// that blocks share a CU and some read while others rank: 2048 rows with 64 alternatives 103 us, 143
 // with a block of 1024 alone on its CU
 template <int DT, int NT, bool TOP>
 __global__ __launch_bounds__(NT, 8) void logprobs_kernel(const void* __restrict__ logits, long ld, int V,
