@@ -54,7 +54,7 @@ struct Teacher {
 // The row stays in the block's registers (16 pieces a thread) between the sums and the gradient, and
 // the block walks rows, reading each piece of its next row as the piece of this row leaves: the
 // loads of one row and the stores of another are in flight while the exponentials are computed.
-// 4096 rows of 128256 bf16 logits: 415-440 us (5.1 TB/s; a copy of the same bytes takes 430), where
+// 4096 rows of 128256 bf16 logits: 443 us (4.7 TB/s; a copy of the same bytes takes 365), where
 // two passes over rows, the second from the caches, take 525 and a block per row without the
 // reads ahead takes 600.  Groups of pieces behind a row's end are jumped over by the whole block:
 // 4096 rows of 4000 bf16 logits take 25 us, and 70 where every thread goes through all sixteen.
@@ -247,12 +247,17 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
       u32x4 o = pack_piece<DT>(f);
       asm volatile("" : "+v"(o));                        // done with b[j] before it is loaded again
       b[j] = load_mine<NT>(rown, j, nfull, tid);
-      char* oj = orow + j * NT * 16;
+      int oj = j * NT * 16;
       asm volatile("" : "+s"(oj));
       if (j * NT + tid < nfull) {
-        u32x4_a2* at = (u32x4_a2*)(oj + (size_t)(u32)(tid * 16));
-        if (keep) *at = o;
-        else __builtin_nontemporal_store(o, at);
+        u32x4_a2* at = (u32x4_a2*)(orow + oj + (size_t)(u32)(tid * 16));
+        if (keep) {
+          *at = o;
+        } else {
+          asm volatile("; past the caches");             // what keeps the two stores from becoming one
+          __builtin_nontemporal_store(o, at);
+          asm volatile("");
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -516,8 +521,10 @@ bool fits_registers(int dt, int V) {
 }
 
 // outputs of more than the last-level cache's 256 MB leave nothing in it for their reader: they are
-// stored past the caches (4096 x 128256 bf16: 436 us against 450)
-constexpr long CACHE_BYTES = 256L << 20;
+// stored past the caches where every row starts on a multiple of 64 bytes (4096 rows of 128256 bf16
+// logits 443 us against 450, of 128288 458 and 464; of 128272, where waves share such pieces, 472 and
+// 468, of 128258 482 and 473)
+constexpr long CACHE_BYTES = 256L << 20, LINE = 64;
 
 }  // namespace
 
@@ -543,7 +550,7 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
   if (mode == KD_FUSED && fits_registers(dt, V)) {
     if (rows == 0) return 0;
     const long bytes = (long)V * (dt == DT_FP32 ? 4 : 2);
-    const int keep = rows * bytes <= CACHE_BYTES;
+    const int keep = rows * bytes <= CACHE_BYTES || (((size_t)out | (size_t)(ldo * (dt == DT_FP32 ? 4 : 2))) & (LINE - 1));
     by_type(dt, [&](auto DTc) {
       auto go = [&](auto NTc, auto Sc, auto Rc) {
         constexpr int DT = decltype(DTc)::value, NT = decltype(NTc)::value, RES = decltype(Sc)::value;
