@@ -16,7 +16,7 @@ NEG = float("-inf")
 
 @pytest.fixture(scope="module", autouse=True)
 def _lib():
-    assert _ext.load(), "HIP library must load on a GPU box"
+    assert _ext.load(), "the HIP library must load"
 
 
 def _x(T, V, dtype, seed=0, pad=0, skip=0):
