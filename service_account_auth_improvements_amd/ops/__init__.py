@@ -348,21 +348,25 @@ def distill_topk_fused(logits, teacher_ids, teacher_logits, scale, temperature=1
 def distill_topk_stats(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None, vocab_start=0,
                        vocab_size=None):
     """:func:`distill_topk_fused` of one vocabulary part (columns [vocab_start, vocab_start + V) of
-    ``vocab_size``; the teacher's ids are global), first half: this part's row statistics [T, 8].
+    ``vocab_size``; the teacher's ids are global), first half: this part's row statistics [T, 9].
     Join the parts' with :func:`distill_topk_join`, then :func:`distill_topk_grad`."""
     return _distill(logits, teacher_ids, teacher_logits, teacher_lse, temperature, 1.0, None, vocab_start, vocab_size,
                     DISTILL_STATS, None, None)[1]
 
 
 def distill_topk_join(parts, temperature=1.0):
-    """Statistics [R, T, 8] of the R parts of a vocabulary -> the whole rows' [T, 8]."""
-    m, s, u, xq, q = parts[..., :5].unbind(-1)
-    M = m.amax(0)
-    # a part (or row) of nothing but -inf: its sums are 0 whatever the shift
-    d = torch.where(torch.isneginf(m) | (m == M), torch.zeros_like(m), m - M)
-    f = torch.exp(d / temperature)
-    student = torch.stack([M, (s * f).sum(0), (u * f).sum(0), (xq + torch.where(q == 0, q, q * d)).sum(0), q.sum(0)], -1)
-    return torch.cat([student, parts[0, :, 5:]], -1)          # the teacher's columns are the same everywhere
+    """Statistics [R, T, 9] of the R parts of a vocabulary -> the whole rows' [T, 9]."""
+    m, s, mo, u, xq, q = parts[..., :6].unbind(-1)
+
+    def shift(m):
+        # a part (or row) of nothing but -inf: its sums are 0 whatever the shift
+        M = m.amax(0)
+        d = torch.where(torch.isneginf(m) | (m == M), torch.zeros_like(m), m - M)
+        return M, d, torch.exp(d / temperature)
+    M, d, f = shift(m)
+    MO, _, fo = shift(mo)
+    student = torch.stack([M, (s * f).sum(0), MO, (u * fo).sum(0), (xq + torch.where(q == 0, q, q * d)).sum(0), q.sum(0)], -1)
+    return torch.cat([student, parts[0, :, 6:]], -1)          # the teacher's columns are the same everywhere
 
 
 def distill_topk_grad(logits, teacher_ids, teacher_logits, stats, scale, temperature=1.0, teacher_lse=None,

@@ -401,7 +401,7 @@ at::Tensor token_logprobs_bwd(const at::Tensor& x, const at::Tensor& tokens, con
 }
 
 // mode 0: loss rows, gradient into out; 1: loss rows of an undivided vocabulary and this part's
-// statistics [T, 8]; 2: loss rows from joined statistics (none with row weights: the backward pass of
+// statistics [T, 9]; 2: loss rows from joined statistics (none with row weights: the backward pass of
 // mode 1), gradient into out.  Returns (loss rows, statistics, gradient); the gradient is empty where
 // it went to out.
 std::tuple<at::Tensor, at::Tensor, at::Tensor> distill_topk(const at::Tensor& x, const at::Tensor& ids, const at::Tensor& z,

@@ -5,14 +5,16 @@
 //   q = exp(z / temperature - lse), r = max(0, 1 - sum q) the teacher's rest  (with it)
 //   loss = sum q (ln q - ln p_id) + r (ln r - ln R),      R = sum of p outside the ids
 //   dx_j = (p_j W - q_j) / temperature          inside,   W = sum q + r
-//   dx_j = p_j (W - r / R) / temperature        outside
+//   dx_j = o_j (W R - r) / temperature          outside,  o_j = p_j / R
 //
 // An entry with a negative id is no entry; a row without entries (or with q = 0 throughout) has
-// loss 0 and gradient 0.  Where the student has no mass outside (R = 0) the rest is left out.  An id
-// at or behind the vocabulary's end makes its row NaN.
+// loss 0 and gradient 0.  Where the student has no mass outside (nothing but -inf) the rest is left
+// out.  An id at or behind the vocabulary's end makes its row NaN.
 //
 // The outside sum is summed over the outside elements, not formed as 1 - sum p_id, which loses
-// everything when the student is sure.
+// everything when the student is sure, and against their own greatest logit mo:  u = sum 2^((x - mo) a),
+// R = u 2^((mo - m) a) / s.  Against the row's, u would be flushed to 0, and 1 / R overflow, from a
+// distance of 87 nats on; so R may vanish, o and ln R = (mo - m) / temperature + ln u - ln s do not.
 #include "logits.h"
 
 using namespace kf;
@@ -25,10 +27,24 @@ constexpr int K_MAX = 256;           // one thread per entry in the smallest blo
 constexpr size_t BITS_MAX = 61440;   // bytes of LDS for a bit per element: 491520 logits
 constexpr int BAD = 0x7fffffff;      // an id behind the vocabulary
 
-// a row's statistics between the two halves: the student's (m, s, outside sum, sum q (x - m), sum q
-// of this part's ids) and the teacher's (greatest z and sum without lse, else 0 and sum q) and the
-// row's state (0 no entries, 1 entries, NaN an id behind the vocabulary)
-enum { ST_M, ST_S, ST_U, ST_XQ, ST_QL, ST_ZM, ST_ZN, ST_LIVE, ST_COLS };
+// a row's statistics between the two halves: the student's (m, s, mo, u, sum q (x - m), sum q of this
+// part's ids) and the teacher's (greatest z and sum without lse, else 0 and sum q) and the row's state
+// (0 no entries, 1 entries, NaN an id behind the vocabulary)
+enum { ST_M, ST_S, ST_MO, ST_U, ST_XQ, ST_QL, ST_ZM, ST_ZN, ST_LIVE, ST_COLS };
+
+// What a row's outside comes to, from its statistics: whether the rest counts, ln R, and
+// k = (W R - r) / u with  dx_j = k 2^((x_j - mo) a) / temperature.  Nothing but -inf outside: k = 0,
+// or NaN where the whole row is nothing else (s = 0).
+struct Outside {
+  bool use;
+  float lnR, k;
+};
+__device__ __forceinline__ Outside outside(float m, float s, float mo, float u, float W, float rest, float a, float inv_temp) {
+  const bool use = rest > 0.f && !(u == 0.f);
+  const float d = mo == -INFINITY ? 0.f : mo - m;
+  const float R = u * __builtin_amdgcn_exp2f(d * a) / s;
+  return {use, d * inv_temp + LN2 * (__log2f(u) - __log2f(s)), (W * R - (use ? rest : 0.f)) / (u == 0.f ? 1.f : u)};
+}
 
 struct Teacher {
   const void* ids;       // int64 or int32 [T, K], rows ldi apart
@@ -82,7 +98,7 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
     float scale_h, float* loss, int keep) {
   constexpr int N = Elem<DT>::N;
   __shared__ float red[5][NT / 64];
-  __shared__ RowStat red3[NT / 64];
+  __shared__ RowStat red3[NT / 64][2];
   __shared__ int head[NT];                               // a thread's own ids: a list through next
   __shared__ int sid[K_MAX], next[K_MAX];
   __shared__ float sq[K_MAX], slq[K_MAX], sx[K_MAX], sqs[K_MAX];
@@ -211,29 +227,30 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
       stat_move<PLAIN>(st, fmaxf(st.m, xt), a);
       stat_add<PLAIN>(st, stat_ref(st.m), xt, a);
     }
+    RowStat so = st;                                     // what lies outside
     if constexpr (REST) {
-      st.u = st.s;
       if (first) {
         const float v = sx[tid];
-        stat_move<SUBSET>(st, fmaxf(st.m, v), a);
+        stat_move<PLAIN>(st, fmaxf(st.m, v), a);
         stat_add<PLAIN>(st, stat_ref(st.m), v, a);
       }
     }
 #pragma unroll
     for (int j = 0; j < RES; ++j) asm volatile("" : "+v"(b[j]));        // unpacked anew below, not kept
     asm volatile("" : "+s"(nfull));                      // nor are the comparisons with it
-    st = block_stat<REST ? SUBSET : PLAIN, NT>(st, a, red3, tid);
-    const float m = st.m, s = st.s, u = st.u;
-    const float L = __log2f(s);
-    const bool use_rest = REST && rest > 0.f && !(u == 0.f);
+    if constexpr (REST) block_stat2<NT>(st, so, a, red3, tid);
+    else st = block_stat<PLAIN, NT>(st, a, red3[0], tid);
+    const float m = st.m, L = __log2f(st.s);
+    const Outside o = REST ? outside(m, st.s, so.m, so.s, W, rest, a, inv_temp) : Outside{};
     if (more && id >= 0 && id < V) x = load1<DT>(rown, id);
     // ---- gradient; each piece of the next row is read as this row's leaves.  ci: 0 without
     // entries, NaN for a bad row
     const bool live = some && !bad;
     const float ci = bad ? quiet_nan() : some ? sc : 0.f;
-    const float k1 = ci * (use_rest ? W - rest * s / u : W), kW = ci * W;
+    const float kW = ci * W, k1 = REST ? ci * o.k : kW;
+    const float ref = REST ? stat_ref(so.m) : m, shift = REST ? 0.f : -L;
     if (tid < ntail) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(xt - m, a, -L));
+      const float p = __builtin_amdgcn_exp2f(fmaf(xt - ref, a, shift));
       store1<DT>(orow, (long)N * nfull + tid, k1 * p);
       xt = load1<DT>(rown, (long)N * nfull + tid);
     }
@@ -243,19 +260,19 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
       float f[N];
       unpack_piece<DT>(b[j], f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = k1 * __builtin_amdgcn_exp2f(fmaf(f[i] - m, a, -L));
-      u32x4 o = pack_piece<DT>(f);
-      asm volatile("" : "+v"(o));                        // done with b[j] before it is loaded again
+      for (int i = 0; i < N; ++i) f[i] = k1 * __builtin_amdgcn_exp2f(fmaf(f[i] - ref, a, shift));
+      u32x4 piece = pack_piece<DT>(f);
+      asm volatile("" : "+v"(piece));                      // done with b[j] before it is loaded again
       b[j] = load_mine<NT>(rown, j, nfull, tid);
       int oj = j * NT * 16;
       asm volatile("" : "+s"(oj));
       if (j * NT + tid < nfull) {
         u32x4_a2* at = (u32x4_a2*)(orow + oj + (size_t)(u32)(tid * 16));
         if (keep) {
-          *at = o;
+          *at = piece;
         } else {
           asm volatile("; past the caches");             // what keeps the two stores from becoming one
-          __builtin_nontemporal_store(o, at);
+          __builtin_nontemporal_store(piece, at);
           asm volatile("");
         }
       }
@@ -270,45 +287,50 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
     const float q = tid < K ? sq[tid] : 0.f;             // entries of q = 0 add nothing, whatever the student gives them
     float l = q != 0.f ? q * (slq[tid] - ((sx[tid] - m) * inv_temp - LN2 * L)) : 0.f;
     l = block_reduce<NT>(l, 0.f, red[4], OpAdd{}, tid);
-    if (use_rest) l += rest * LN2 * (__log2f(rest) - (__log2f(u) - L));
+    if (o.use) l += rest * (LN2 * __log2f(rest) - o.lnR);
     if (tid == 0) loss[r] = bad ? quiet_nan() : some ? l : 0.f;
   }
 }
 
 // ---------------------------------------------------------------- statistics: one block per row
+// the sums of a thread's pieces; REST: of what lies outside, and the ids' elements go into `in`
 template <int DT, int NT, bool REST>
-__device__ __forceinline__ RowStat walk_sums(const char* row, int V, float a, const u32* bits) {
+__device__ __forceinline__ RowStat walk_sums(const char* row, int V, float a, const u32* bits, RowStat& in) {
   constexpr int N = Elem<DT>::N, UN = 4;
   const int nfull = V / N;
   RowStat st = stat_empty();
+  in = stat_empty();
   float f[UN][N];
   auto eat = [&](int c0, int n) {
+    if constexpr (REST) {
+#pragma unroll
+      for (int j = 0; j < UN; ++j) {
+        if (j >= n) continue;
+        const long e = (long)N * (c0 + j * NT);
+        const u32 here = e < V ? bits[e >> 5] >> (e & 31) & ((1u << N) - 1) : 0u;
+        if (here == 0) continue;                         // few pieces hold an id
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if ((here >> i & 1) == 0) continue;
+          stat_move<PLAIN>(in, fmaxf(in.m, f[j][i]), a);
+          stat_add<PLAIN>(in, stat_ref(in.m), f[j][i], a);
+          f[j][i] = -INFINITY;
+        }
+      }
+    }
     float bm = st.m;
 #pragma unroll
     for (int j = 0; j < UN; ++j)
       if (j < n) bm = fmaxf(bm, max_piece<DT>(f[j]));
-    if (bm != st.m) stat_move<REST ? SUBSET : PLAIN>(st, bm, a);
+    if (bm != st.m) stat_move<PLAIN>(st, bm, a);
     const float ref = stat_ref(st.m);
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
       if (j >= n) continue;
       float part = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        f[j][i] = __builtin_amdgcn_exp2f((f[j][i] - ref) * a);
-        part += f[j][i];
-      }
+      for (int i = 0; i < N; ++i) part += __builtin_amdgcn_exp2f((f[j][i] - ref) * a);
       st.s += part;
-      if constexpr (REST) {
-        const long e = (long)N * (c0 + j * NT);
-        const u32 in = e < V ? bits[e >> 5] >> (e & 31) & ((1u << N) - 1) : 0u;
-        if (in) {                                        // few pieces hold an id
-          part = 0.f;
-#pragma unroll
-          for (int i = 0; i < N; ++i) part += (in >> i & 1) ? 0.f : f[j][i];
-        }
-        st.u += part;
-      }
     }
   };
   for (int c = threadIdx.x; c < nfull; c += UN * NT) {
@@ -335,7 +357,7 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
                                                               long vstart, Teacher te, float temp,
                                                               float* __restrict__ loss, float* __restrict__ stats) {
   __shared__ float red[6][NT / 64];
-  __shared__ RowStat red3[NT / 64];
+  __shared__ RowStat red3[NT / 64][2];
   extern __shared__ u32 bits[];                          // REST: one bit per element
   const float inv_temp = 1.f / temp, a = LOG2E * inv_temp;
   const long r = blockIdx.x;
@@ -370,7 +392,18 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
     if (tid < ST_COLS) st_row[tid] = v;
     return;
   }
-  RowStat st = block_stat<REST ? SUBSET : PLAIN, NT>(walk_sums<DT, NT, REST>(row, V, a, bits), a, red3, tid);
+  RowStat in, so = walk_sums<DT, NT, REST>(row, V, a, bits, in), st = so;
+  if constexpr (REST) {
+    // the ids' elements join the rest of the row
+    const float mn = fmaxf(st.m, in.m);
+    stat_move<PLAIN>(st, mn, a);
+    stat_move<PLAIN>(in, mn, a);
+    st.s += in.s;
+    block_stat2<NT>(st, so, a, red3, tid);
+  } else {
+    st = block_stat<PLAIN, NT>(st, a, red3[0], tid);
+    so = stat_empty();
+  }
   const float L = __log2f(st.s);
   // entries of q = 0 add nothing, whatever the student gives them
   const bool use = mine && q != 0.f;
@@ -378,10 +411,11 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
   const float xq = block_reduce<NT>(use ? q * (x - stat_ref(st.m)) : 0.f, 0.f, red[3], OpAdd{}, tid);
   const float ql = block_reduce<NT>(mine ? q : 0.f, 0.f, red[4], OpAdd{}, tid);
   float l = block_reduce<NT>(use ? q * (lq - ((x - st.m) * inv_temp - LN2 * L)) : 0.f, 0.f, red[5], OpAdd{}, tid);
-  if (REST && rest > 0.f && !(st.u == 0.f)) l += rest * LN2 * (__log2f(rest) - (__log2f(st.u) - L));
+  const Outside o = REST ? outside(st.m, st.s, so.m, so.s, n + rest, rest, a, inv_temp) : Outside{};
+  if (o.use) l += rest * (LN2 * __log2f(rest) - o.lnR);
   if (tid == 0) {
     loss[r] = l;
-    const float row_stats[ST_COLS] = {st.m, st.s, st.u, xq, ql, stat_ref(zm), n, 1.f};
+    const float row_stats[ST_COLS] = {st.m, st.s, so.m, so.s, xq, ql, stat_ref(zm), n, 1.f};
 #pragma unroll
     for (int i = 0; i < ST_COLS; ++i) st_row[i] = row_stats[i];
   }
@@ -418,7 +452,7 @@ __global__ __launch_bounds__(GRAD_NT) void distill_grad_kernel(const void* logit
   const bool has_tail = part == parts - 1 && tail < V;
   const float xt = has_tail ? load1<DT>(row, tail) : 0.f;
   const float* st = stats + r * ST_COLS;
-  const float live = st[ST_LIVE], m = st[ST_M], s = st[ST_S], u = st[ST_U], n = st[ST_ZN], zm = st[ST_ZM];
+  const float live = st[ST_LIVE], m = st[ST_M], s = st[ST_S], n = st[ST_ZN], zm = st[ST_ZM];
   const bool all = loss && part == 0;                    // every entry counts in the loss
   int id;
   float z;
@@ -484,26 +518,26 @@ __global__ __launch_bounds__(GRAD_NT) void distill_grad_kernel(const void* logit
     sqs[tid] = qs;
   }
   lds_barrier();
-  const bool use_rest = REST && rest > 0.f && !(u == 0.f);
+  const Outside o = REST ? outside(m, s, st[ST_MO], st[ST_U], W, rest, a, inv_temp) : Outside{};
   const float sc = (rows ? rows[r] : 1.f) * (scale_ptr ? scale_ptr[0] : scale_h) * inv_temp;
-  const float k1 = sc * (use_rest ? W - rest * s / u : W);
+  const float k1 = sc * (REST ? o.k : W), ref = REST ? stat_ref(st[ST_MO]) : m, shift = REST ? 0.f : -L;
 #pragma unroll
   for (int j = 0; j < GRAD_UN; ++j) {
     if (c0 + j * GRAD_NT >= nfull) continue;
     float f[N];
     unpack_piece<DT>(v[j], f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = k1 * __builtin_amdgcn_exp2f(fmaf(f[i] - m, a, -L));
+    for (int i = 0; i < N; ++i) f[i] = k1 * __builtin_amdgcn_exp2f(fmaf(f[i] - ref, a, shift));
     store_piece<DT>(orow, c0 + j * GRAD_NT, f);
   }
-  if (has_tail) store1<DT>(orow, tail, k1 * __builtin_amdgcn_exp2f(fmaf(xt - m, a, -L)));
+  if (has_tail) store1<DT>(orow, tail, k1 * __builtin_amdgcn_exp2f(fmaf(xt - ref, a, shift)));
   // each by the thread that stored around it, behind that store
   asm volatile("" ::: "memory");
   for (int h = head[tid]; h; h = next[h - 1])
     store1<DT>(orow, scol[h - 1], sc * fmaf(W, __builtin_amdgcn_exp2f(fmaf(sx[h - 1] - m, a, -L)), -sqs[h - 1]));
   if (all) {
     float l = block_reduce<GRAD_NT>(q != 0.f ? q * (lq + LN2 * L) : 0.f, 0.f, red, OpAdd{}, tid) - inv_temp * st[ST_XQ];
-    if (use_rest) l += rest * LN2 * (__log2f(rest) - (__log2f(u) - L));
+    if (o.use) l += rest * (LN2 * __log2f(rest) - o.lnR);
     if (tid == 0) loss[r] = l;
   }
 }

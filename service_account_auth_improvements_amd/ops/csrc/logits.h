@@ -196,11 +196,10 @@ __device__ __forceinline__ float block_reduce(float v, float neutral, float* red
   return lane_value(row_reduce(l < NT / 64 ? red[l] : neutral, neutral, op), 15);
 }
 
-// Running softmax of a row part: m = greatest logit, s = sum 2^((x-m) a), and u, a second sum of the
-// same weights: sum (x-m) 2^((x-m) a) (MOMENT, for the entropy) or the sum over some of the elements
-// (SUBSET).  An empty part is {-inf, 0, 0}, and so is one whose logits are all -inf.  A NaN or +inf
-// logit makes s NaN.
-enum { MOMENT = 0, SUBSET = 1, PLAIN = 2 };
+// Running softmax of a row part: m = greatest logit, s = sum 2^((x-m) a), and for the entropy (MOMENT)
+// u = sum (x-m) 2^((x-m) a).  An empty part is {-inf, 0, 0}, and so is one whose logits are all -inf.
+// A NaN or +inf logit makes s NaN.
+enum { MOMENT = 0, PLAIN = 1 };
 struct RowStat {
   float m, s, u;
 };
@@ -216,7 +215,6 @@ __device__ __forceinline__ void stat_move(RowStat& r, float mn, float a) {
   const float d = r.m == -INFINITY ? 0.f : fmaxf(r.m - mn, FAR);
   const float f = __builtin_amdgcn_exp2f(d * a);
   if constexpr (KIND == MOMENT) r.u = f * fmaf(d, r.s, r.u);
-  if constexpr (KIND == SUBSET) r.u *= f;
   r.s *= f;
   r.m = mn;
 }
@@ -244,6 +242,18 @@ __device__ __forceinline__ RowStat block_stat(RowStat r, float a, RowStat* red, 
   lds_barrier();
   const int l = tid & 15;
   return lanes_stat<KIND, 16>(l < NT / 64 ? red[l] : stat_empty(), a);
+}
+
+// two parts at once
+template <int NT>
+__device__ __forceinline__ void block_stat2(RowStat& p, RowStat& q, float a, RowStat (*red)[2], int tid) {
+  p = lanes_stat<PLAIN, 64>(p, a);
+  q = lanes_stat<PLAIN, 64>(q, a);
+  if ((tid & 63) == 0) { red[tid >> 6][0] = p; red[tid >> 6][1] = q; }
+  lds_barrier();
+  const int l = tid & 15;
+  p = lanes_stat<PLAIN, 16>(l < NT / 64 ? red[l][0] : stat_empty(), a);
+  q = lanes_stat<PLAIN, 16>(l < NT / 64 ? red[l][1] : stat_empty(), a);
 }
 
 constexpr long ROWS_PER_LAUNCH = 1 << 20;   // a launch holds less than 2^32 threads

@@ -178,7 +178,7 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp, dentropy, temperat
 
 
 def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_start, vocab_size, mode, stats, out):
-    """ops.distill_topk_*: mode 0 loss rows and gradient; 1 loss rows and statistics [T, 8]; 2 loss rows
+    """ops.distill_topk_*: mode 0 loss rows and gradient; 1 loss rows and statistics [T, 9]; 2 loss rows
     and gradient from joined statistics.  Returns (loss, statistics, gradient)."""
     op = "distill_topk"
     _check_logits(logits, temperature, op)
@@ -202,7 +202,7 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
     if rows is not None:
         _check_rows(rows, logits, (), op, "row weights")
     if mode == 2:
-        _check_rows(stats, logits, (8,), op, "stats")
+        _check_rows(stats, logits, (9,), op, "stats")
     _need(mode != 1 or out is None, f"{op}: out goes with a gradient")
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype)
@@ -231,32 +231,39 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
     x = logits.float()
     inside = torch.zeros(T, V + 1, dtype=torch.bool).scatter_(1, col, True)[:, :V]
     xk = torch.cat([x, torch.zeros(T, 1)], 1).gather(1, col)
+    xo = x.masked_fill(inside, float("-inf"))                          # what lies outside, against its own greatest
+
+    def sums(v):
+        m = v.amax(1, keepdim=True)
+        return m, torch.exp(torch.where(torch.isneginf(m), v, v - m) / temperature).sum(1, keepdim=True)
     if mode != 2:
-        m = x.amax(1, keepdim=True)
-        d = torch.where(torch.isneginf(m), x, x - m)
-        e = torch.exp(d / temperature)
-        s, u = e.sum(1, keepdim=True), torch.where(inside, zero, e).sum(1, keepdim=True)
-        if lse is None:
-            u = torch.zeros_like(s)
+        m, s = sums(x)
+        mo, u = sums(xo) if lse is not None else (torch.full_like(m, float("-inf")), torch.zeros_like(m))
         ok = here & (q != 0)
         xq = torch.where(ok, q * (xk - torch.where(torch.isneginf(m), 0.0, m)), zero).sum(1, keepdim=True)
-        # the student's (max, sum, outside sum, sum q (x - max), sum q here), the teacher's (max and sum
-        # of the softmax, or 0 and sum q) and whether the row has entries
+        # the student's (max, sum, outside max, outside sum, sum q (x - max), sum q here), the teacher's
+        # (max and sum of the softmax, or 0 and sum q) and whether the row has entries
         tm, tn = (mz * temperature, n) if lse is None else (torch.zeros(T, 1), q.sum(1, keepdim=True))
-        part = torch.cat([m, s, u, xq, torch.where(here, q, zero).sum(1, keepdim=True), tm, tn, torch.ones(T, 1)], 1)
+        part = torch.cat([m, s, mo, u, xq, torch.where(here, q, zero).sum(1, keepdim=True), tm, tn, torch.ones(T, 1)], 1)
     else:
-        m, s, u, xq = stats[:, :4].split(1, 1)
+        m, s, mo, u, xq = stats[:, :5].split(1, 1)
         part = None
     logs = torch.log(s)
+    # ln of the mass outside
+    do = torch.where(torch.isneginf(mo), zero, mo - m)
+    lnR = do / temperature + torch.log(u) - logs
     live = (rest.unsqueeze(1) > 0) & (u != 0)
     loss = torch.where(q != 0, q * (lq + logs), zero).sum(1) - (xq / temperature).squeeze(1)
     r1 = rest.unsqueeze(1)
-    loss = loss + torch.where(live, r1 * (torch.log(r1) - (torch.log(u) - logs)), zero).squeeze(1)
+    loss = loss + torch.where(live, r1 * (torch.log(r1) - lnR), zero).squeeze(1)
     loss = loss.masked_fill(~some, 0.0).masked_fill(bad, nan)
     if mode == 1:
         return loss, part.masked_fill(~some.unsqueeze(1), 0.0).masked_fill(bad.unsqueeze(1), nan), None
     p = torch.exp((x - m) / temperature - logs)
-    dx = torch.where(inside, p * W, p * torch.where(live, W - r1 * s / u, W))
+    # outside: p W - o r with o the softmax there; R itself may vanish
+    o = torch.exp(torch.where(torch.isneginf(mo), xo, xo - mo) / temperature) / torch.where(u == 0, torch.ones_like(u), u)
+    dx = torch.where(inside, p, p if lse is None else o * (u * torch.exp(do / temperature) / s)) * W
+    dx = dx - torch.where(live, o * r1, zero)
     dx = torch.cat([dx, torch.zeros(T, 1)], 1).scatter_add_(1, col, torch.where(here, -q, zero))[:, :V]
     dx = dx * (scale_h / temperature) * (1.0 if rows is None else rows.unsqueeze(1))
     out.copy_(dx.masked_fill(~some.unsqueeze(1), 0.0).masked_fill(bad.unsqueeze(1), nan))
