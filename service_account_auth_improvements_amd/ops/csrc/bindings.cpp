@@ -82,7 +82,7 @@ int kf_distill_stats_cols();
 int kf_distill_needs_stats(int, int);
 long kf_distill_rest_v_max();
 int kf_distill_topk(const void*, int, long, void*, long, long, int, long, long, const void*, int, long, const void*, int,
-                    long, const float*, int, float, const float*, float, const float*, float*, float*, int, hipStream_t);
+                    long, const float*, int, double, const float*, float, const float*, float*, float*, int, hipStream_t);
 long kf_car_header_bytes();
 int kf_car_alloc(long, void**, void*);
 int kf_car_open(const void*, void**);
@@ -453,7 +453,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> distill_topk(const at::Tensor& x,
   const at::Tensor& d = out.has_value() ? *out : fresh;
   check_rc(kf_distill_topk(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), T, (int)V, vocab_start, vocab_size, ids.data_ptr(),
                            ids.scalar_type() == at::kInt ? 1 : 0, ids.stride(0), z.data_ptr(), zt, z.stride(0),
-                           lse.has_value() ? lse->data_ptr<float>() : nullptr, (int)K, (float)temperature,
+                           lse.has_value() ? lse->data_ptr<float>() : nullptr, (int)K, temperature,
                            scale.has_value() ? scale->data_ptr<float>() : nullptr, (float)scale_h,
                            rows.has_value() ? rows->data_ptr<float>() : nullptr,
                            want_loss ? loss.data_ptr<float>() : nullptr, st, (int)mode,

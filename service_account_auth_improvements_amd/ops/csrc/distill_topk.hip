@@ -28,9 +28,9 @@ constexpr size_t BITS_MAX = 61440;   // bytes of LDS for a bit per element: 4915
 constexpr int BAD = 0x7fffffff;      // an id behind the vocabulary
 
 // a row's statistics between the two halves: the student's (m, s, mo, u, sum q (x - m), sum q of this
-// part's ids) and the teacher's (greatest z and sum without lse, else 0 and sum q) and the row's state
+// part's ids) and the teacher's (greatest z and sum without lse, else r and sum q) and the row's state
 // (0 no entries, 1 entries, NaN an id behind the vocabulary)
-enum { ST_M, ST_S, ST_MO, ST_U, ST_XQ, ST_QL, ST_ZM, ST_ZN, ST_LIVE, ST_COLS };
+enum { ST_M, ST_S, ST_MO, ST_U, ST_XQ, ST_QL, ST_ZM, ST_ZN, ST_LIVE, ST_COLS, ST_REST = ST_ZM };
 
 // What a row's outside comes to, from its statistics: whether the rest counts, ln R, and
 // k = (W R - r) / u with  dx_j = k 2^((x_j - mo) a) / temperature.  Nothing but -inf outside: k = 0,
@@ -50,6 +50,7 @@ struct Teacher {
   const void* ids;       // int64 or int32 [T, K], rows ldi apart
   const void* z;         // logits' row of any of the three types, rows ldz apart
   const float* lse;      // [T] or null
+  double inv_temp;
   long ldi, ldz, vocab;
   int ids32, zt, K;
   // entry k of row r: -1 none, BAD behind the vocabulary
@@ -62,6 +63,15 @@ struct Teacher {
       id = i < 0 ? -1 : i >= vocab ? BAD : (int)i;
     }
     if (id < 0) v = -INFINITY;
+  }
+  // q against the teacher's whole mass, and ln q.  In 64 bits: r = 1 - sum q is often small, and at
+  // r = 1e-6 would be off by some per cent, and the outside's gradient with it, were q an fp32 exponential.
+  __device__ __forceinline__ double mass(long r, int id, float v, float& lq) const {
+    lq = -INFINITY;
+    if (id < 0) return 0.0;
+    const double l = (double)v * inv_temp - (double)lse[r];
+    lq = (float)l;
+    return exp(l);
   }
 };
 
@@ -102,6 +112,7 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
   __shared__ int head[NT];                               // a thread's own ids: a list through next
   __shared__ int sid[K_MAX], next[K_MAX];
   __shared__ float sq[K_MAX], slq[K_MAX], sx[K_MAX], sqs[K_MAX];
+  __shared__ double redq[NT / 64];
   const float inv_temp = 1.f / temp, a = LOG2E * inv_temp;
   const int tid0 = threadIdx.x, K = te.K;
   const int nfull0 = V / N, ntail = V % N;
@@ -135,12 +146,11 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
     {
       float lq, q;
       if constexpr (REST) {
-        lq = fmaf(z, inv_temp, -te.lse[r]);
-        q = id >= 0 ? __builtin_amdgcn_exp2f(lq * LOG2E) : 0.f;
-        const float Q = block_reduce<NT>(q, 0.f, red[1], OpAdd{}, tid);
-        some = !(Q == 0.f);
-        rest = fmaxf(1.f - Q, 0.f);
-        W = Q + rest;
+        const double qd = te.mass(r, id, z, lq), Q = block_sum<NT>(qd, redq, tid);
+        q = (float)qd;
+        some = !(Q == 0.0);
+        rest = (float)fmax(1.0 - Q, 0.0);
+        W = (float)Q + rest;
       } else {
         const float zm = block_reduce<NT>(z, -INFINITY, red[1], OpMax{}, tid);
         z -= stat_ref(zm);
@@ -358,6 +368,7 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
                                                               float* __restrict__ loss, float* __restrict__ stats) {
   __shared__ float red[6][NT / 64];
   __shared__ RowStat red3[NT / 64][2];
+  __shared__ double redq[NT / 64];
   extern __shared__ u32 bits[];                          // REST: one bit per element
   const float inv_temp = 1.f / temp, a = LOG2E * inv_temp;
   const long r = blockIdx.x;
@@ -371,12 +382,14 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
   if constexpr (REST)
     for (int i = tid; i < (V + 31) / 32; i += NT) bits[i] = 0;
   const bool bad = block_reduce<NT>(id == BAD ? 1.f : 0.f, 0.f, red[0], OpMax{}, tid) != 0.f;
+  bool some;
   if constexpr (REST) {
-    lq = fmaf(z, inv_temp, -te.lse[r]);
-    q = id >= 0 ? __builtin_amdgcn_exp2f(lq * LOG2E) : 0.f;
     if (mine) atomicOr(&bits[(id - vstart) >> 5], 1u << ((id - vstart) & 31));
-    n = block_reduce<NT>(q, 0.f, red[1], OpAdd{}, tid);
-    rest = fmaxf(1.f - n, 0.f);
+    const double qd = te.mass(r, id, z, lq), Q = block_sum<NT>(qd, redq, tid);
+    q = (float)qd;
+    n = (float)Q;
+    some = !(Q == 0.0);
+    rest = (float)fmax(1.0 - Q, 0.0);
   } else {
     zm = block_reduce<NT>(z, -INFINITY, red[1], OpMax{}, tid);
     z -= stat_ref(zm);
@@ -384,9 +397,10 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
     n = block_reduce<NT>(q, 0.f, red[2], OpAdd{}, tid);
     lq = z * inv_temp - LN2 * __log2f(n);
     q = n == 0.f ? 0.f : q / n;
+    some = !(n == 0.f);
   }
   float* st_row = stats + r * ST_COLS;
-  if (n == 0.f || bad) {
+  if (!some || bad) {
     const float v = bad ? quiet_nan() : 0.f;
     if (tid == 0) loss[r] = v;
     if (tid < ST_COLS) st_row[tid] = v;
@@ -415,7 +429,7 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
   if (o.use) l += rest * (LN2 * __log2f(rest) - o.lnR);
   if (tid == 0) {
     loss[r] = l;
-    const float row_stats[ST_COLS] = {st.m, st.s, so.m, so.s, xq, ql, stat_ref(zm), n, 1.f};
+    const float row_stats[ST_COLS] = {st.m, st.s, so.m, so.s, xq, ql, REST ? rest : stat_ref(zm), n, 1.f};
 #pragma unroll
     for (int i = 0; i < ST_COLS; ++i) st_row[i] = row_stats[i];
   }
@@ -473,11 +487,10 @@ __global__ __launch_bounds__(GRAD_NT) void distill_grad_kernel(const void* logit
   const bool mine = id >= 0 && col >= (long)N * p0 && col < min((long)V, part == parts - 1 ? (long)V : (long)N * (p0 + GRAD_NT * GRAD_UN));
   const float x = mine ? load1<DT>(row, col) : 0.f;
   const float L = __log2f(s);
-  float lq, q, rest = 0.f, W = 1.f;
+  float lq = 0.f, q, rest = 0.f, W = 1.f;
   if constexpr (REST) {
-    lq = fmaf(z, inv_temp, -te.lse[r]);
-    q = id >= 0 ? __builtin_amdgcn_exp2f(lq * LOG2E) : 0.f;
-    rest = fmaxf(1.f - n, 0.f);
+    q = mine || all ? (float)te.mass(r, id, z, lq) : 0.f;
+    rest = st[ST_REST];
     W = n + rest;
   } else {
     z -= zm;
@@ -575,10 +588,11 @@ int kf_distill_needs_stats(int dt, int V) { return fits_registers(dt, V) ? 0 : 1
 // undivided vocabulary; 2: gradient (and loss rows) from joined statistics
 int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, long rows, int V, long vstart, long vtotal,
                     const void* ids, int ids32, long ldi, const void* z, int zt, long ldz, const float* lse, int K,
-                    float temp, const float* scale_ptr, float scale_h, const float* row_scale, float* loss, float* stats,
+                    double temperature, const float* scale_ptr, float scale_h, const float* row_scale, float* loss, float* stats,
                     int mode, hipStream_t s) {
   if (V < 1 || K < 0 || K > K_MAX || dt < DT_BF16 || dt > DT_FP32 || zt < DT_BF16 || zt > DT_FP32) return 1;
-  const Teacher te{ids, z, lse, ldi, ldz, vtotal, ids32, zt, K};
+  const Teacher te{ids, z, lse, 1.0 / temperature, ldi, ldz, vtotal, ids32, zt, K};
+  const float temp = (float)temperature;
   const size_t lds = lse ? ((size_t)V + 31) / 32 * 4 : 0;
   if (lds > BITS_MAX) return 2;
   if (mode == KD_FUSED && fits_registers(dt, V)) {

@@ -195,6 +195,37 @@ __device__ __forceinline__ float block_reduce(float v, float neutral, float* red
   const int l = tid & 15;
   return lane_value(row_reduce(l < NT / 64 ? red[l] : neutral, neutral, op), 15);
 }
+// the same sum in 64 bits
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+  const u32x2 p = __builtin_bit_cast(u32x2, v);
+  u32x2 q;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) q[i] = (u32)__builtin_amdgcn_update_dpp(0, (int)p[i], CTRL, ROWS, 0xf, false);
+  return v + __builtin_bit_cast(double, q);
+}
+__device__ __forceinline__ double row_sum(double v) {
+  v = dpp_add<0x111, 0xf>(v);
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  return dpp_add<0x118, 0xf>(v);
+}
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  u32x2 p = __builtin_bit_cast(u32x2, v);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) p[i] = (u32)__builtin_amdgcn_readlane((int)p[i], lane);
+  return __builtin_bit_cast(double, p);
+}
+template <int NT>
+__device__ __forceinline__ double block_sum(double v, double* red, int tid) {
+  v = row_sum(v);
+  v = dpp_add<0x142, 0xa>(v);
+  v = lane_value(dpp_add<0x143, 0xc>(v), 63);
+  if ((tid & 63) == 0) red[tid >> 6] = v;
+  lds_barrier();
+  const int l = tid & 15;
+  return lane_value(row_sum(l < NT / 64 ? red[l] : 0.0), 15);
+}
 
 // Running softmax of a row part: m = greatest logit, s = sum 2^((x-m) a), and for the entropy (MOMENT)
 // u = sum (x-m) 2^((x-m) a).  An empty part is {-inf, 0, 0}, and so is one whose logits are all -inf.

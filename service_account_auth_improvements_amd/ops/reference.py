@@ -223,11 +223,13 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
         q = torch.where(n == 0, n, q / n)
         rest = torch.zeros(T)
     else:
-        lq = zt - lse.unsqueeze(1)
-        q = torch.where(has, torch.exp(lq), zero)
+        # in 64 bits, as the rest is often small
+        lq = torch.where(has, z.double() / temperature, float("-inf")) - lse.double().unsqueeze(1)
+        q = torch.where(has, torch.exp(lq), 0.0)
         rest = (1 - q.sum(1)).clamp(min=0)
     some = (q != 0).any(1)
-    W = (q.sum(1) + rest).unsqueeze(1)
+    W = (q.sum(1) + rest).float().unsqueeze(1)
+    lq, q, rest = lq.float(), q.float(), rest.float()
     x = logits.float()
     inside = torch.zeros(T, V + 1, dtype=torch.bool).scatter_(1, col, True)[:, :V]
     xk = torch.cat([x, torch.zeros(T, 1)], 1).gather(1, col)
@@ -242,8 +244,8 @@ def distill_topk(logits, ids, z, lse, temperature, scale, scale_h, rows, vocab_s
         ok = here & (q != 0)
         xq = torch.where(ok, q * (xk - torch.where(torch.isneginf(m), 0.0, m)), zero).sum(1, keepdim=True)
         # the student's (max, sum, outside max, outside sum, sum q (x - max), sum q here), the teacher's
-        # (max and sum of the softmax, or 0 and sum q) and whether the row has entries
-        tm, tn = (mz * temperature, n) if lse is None else (torch.zeros(T, 1), q.sum(1, keepdim=True))
+        # (max and sum of the softmax, or rest and sum q) and whether the row has entries
+        tm, tn = (mz * temperature, n) if lse is None else (rest.unsqueeze(1), q.sum(1, keepdim=True))
         part = torch.cat([m, s, mo, u, xq, torch.where(here, q, zero).sum(1, keepdim=True), tm, tn, torch.ones(T, 1)], 1)
     else:
         m, s, mo, u, xq = stats[:, :5].split(1, 1)

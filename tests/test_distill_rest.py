@@ -141,3 +141,27 @@ def test_gradient_by_differences():
     _, d = ops.distill_topk_fused(x.float(), ids, z, 1.0, 1.0, lse)
     # the difference's own error is step^2, its rounding 1e-14 / step; x is rounded to fp32: 110 * 2^-24 on the logits
     oracle.close(d, num, 3e-5, "difference")
+
+
+def _small_rest(device, V, dtype, zt, temperature):
+    """Teachers that leave next to nothing, to students that have still less there: the outside's gradient
+    is the rest's, and as exact as any other."""
+    T, K = 6, 7
+    x, ids, z, _ = _case(T, V, K, dtype, temperature, [25.0, 40.0])
+    z = z.to(zt)
+    full = torch.logsumexp(z.double() / temperature, 1)
+    lse = (full + torch.tensor([1e-6, 1e-5, 1e-4, 3e-6, 1e-6, 0.0]).double()).float()
+    lse[5] = float(full[5].float()) * (1 - 1e-6) if full[5] > 0 else float(full[5].float()) * (1 + 1e-6)    # entries above one: no rest
+    _hold(device, x, ids, z, temperature, lse, far=80.0)
+
+
+@pytest.mark.parametrize("V,dtype,zt,temperature", [(1000, F32, F32, 1.0), (300, BF16, BF16, 0.7), (5000, F32, FP16, 0.1)])
+def test_small_rest(V, dtype, zt, temperature):
+    _small_rest("cpu", V, dtype, zt, temperature)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,dtype,zt,temperature", [(1000, F32, F32, 1.0), (300, BF16, BF16, 0.7), (5000, F32, FP16, 0.1), (40000, BF16, F32, 1.3),
+                                                    (150001, F32, BF16, 1.0)])
+def test_small_rest_gpu(V, dtype, zt, temperature):
+    _small_rest("cuda:0", V, dtype, zt, temperature)
