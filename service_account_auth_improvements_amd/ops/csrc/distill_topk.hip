@@ -32,18 +32,34 @@ constexpr int BAD = 0x7fffffff;      // an id behind the vocabulary
 // (0 no entries, 1 entries, NaN an id behind the vocabulary)
 enum { ST_M, ST_S, ST_MO, ST_U, ST_XQ, ST_QL, ST_ZM, ST_ZN, ST_LIVE, ST_COLS, ST_REST = ST_ZM };
 
-// What a row's outside comes to, from its statistics: whether the rest counts, ln R, and
-// k = (W R - r) / u with  dx_j = k 2^((x_j - mo) a) / temperature.  Nothing but -inf outside: k = 0,
-// or NaN where the whole row is nothing else (s = 0).
-struct Outside {
-  bool use;
-  float lnR, k;
-};
-__device__ __forceinline__ Outside outside(float m, float s, float mo, float u, float W, float rest, float a, float inv_temp) {
-  const bool use = rest > 0.f && !(u == 0.f);
-  const float d = mo == -INFINITY ? 0.f : mo - m;
-  const float R = u * __builtin_amdgcn_exp2f(d * a) / s;
-  return {use, d * inv_temp + LN2 * (__log2f(u) - __log2f(s)), (W * R - (use ? rest : 0.f)) / (u == 0.f ? 1.f : u)};
+// k = (W R - r) / u, with  dx_j = k 2^((x_j - mo) a) / temperature  outside.  u and s are 0 (nothing but
+// -inf), 1 or more, or NaN; k is 0 where u is, and NaN where s is 0.
+__device__ __forceinline__ float outside_factor(float m, float s, float mo, float u, float W, float rest, float a) {
+  const float R = u * __builtin_amdgcn_exp2f((mo - m) * a) * __builtin_amdgcn_rcpf(s);
+  return (W * R - (u == 0.f ? 0.f : rest)) * __builtin_amdgcn_rcpf(fmaxf(u, 1.f));
+}
+// r (ln r - ln R): the rest's share of the loss
+__device__ __forceinline__ float rest_loss(float m, float L, float mo, float u, float rest, float inv_temp) {
+  if (!(rest > 0.f) || u == 0.f) return 0.f;
+  return rest * (LN2 * (__log2f(rest) - __log2f(u) + L) - (mo - m) * inv_temp);
+}
+
+// e^x in 64 bits, to a relative 1e-12: (e^(f / 8))^8 2^n with x = n ln 2 + f and six terms of the series.
+// It needs few constants: those of exp() would take 24 scalar registers from row to row, and one of the
+// fused kernel's would be spilled.
+__device__ __forceinline__ double exp64(double x) {
+  x = x < -800.0 ? -800.0 : x > 800.0 ? 800.0 : x;       // 0 and infinity; NaN passes
+  const double n = rint(x * 1.4426950408889634);
+  const double g = ldexp(fma(n, -0.69314718055994531, x), -3);
+  double p = fma(g, 1.0 / 720, 1.0 / 120);
+  p = fma(g, p, 1.0 / 24);
+  p = fma(g, p, 1.0 / 6);
+  p = fma(g, p, 0.5);
+  p = fma(g, p, 1.0);
+  p = fma(g, p, 1.0);
+  p *= p;
+  p *= p;
+  return ldexp(p * p, (int)n);
 }
 
 struct Teacher {
@@ -71,7 +87,7 @@ struct Teacher {
     if (id < 0) return 0.0;
     const double l = (double)v * inv_temp - (double)lse[r];
     lq = (float)l;
-    return exp(l);
+    return exp64(l);
   }
 };
 
@@ -114,7 +130,7 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
   __shared__ float sq[K_MAX], slq[K_MAX], sx[K_MAX], sqs[K_MAX];
   __shared__ double redq[NT / 64];
   const float inv_temp = 1.f / temp, a = LOG2E * inv_temp;
-  const int tid0 = threadIdx.x, K = te.K;
+  const int tid0 = threadIdx.x, K = te.K, kwaves = (K + 63) / 64;      // waves whose threads hold entries
   const int nfull0 = V / N, ntail = V % N;
   const float sc = (scale_ptr ? scale_ptr[0] : scale_h) * inv_temp;
   auto row_at = [&](long r) { return (const char*)logits + r * ld * Elem<DT>::bytes; };
@@ -146,7 +162,7 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
     {
       float lq, q;
       if constexpr (REST) {
-        const double qd = te.mass(r, id, z, lq), Q = block_sum<NT>(qd, redq, tid);
+        const double qd = te.mass(r, id, z, lq), Q = block_sum(qd, kwaves, redq, tid);
         q = (float)qd;
         some = !(Q == 0.0);
         rest = (float)fmax(1.0 - Q, 0.0);
@@ -248,16 +264,15 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
 #pragma unroll
     for (int j = 0; j < RES; ++j) asm volatile("" : "+v"(b[j]));        // unpacked anew below, not kept
     asm volatile("" : "+s"(nfull));                      // nor are the comparisons with it
-    if constexpr (REST) block_stat2<NT>(st, so, a, red3, tid);
+    if constexpr (REST) block_stat2<NT>(st, so, kwaves, a, red3, tid);
     else st = block_stat<PLAIN, NT>(st, a, red3[0], tid);
     const float m = st.m, L = __log2f(st.s);
-    const Outside o = REST ? outside(m, st.s, so.m, so.s, W, rest, a, inv_temp) : Outside{};
     if (more && id >= 0 && id < V) x = load1<DT>(rown, id);
     // ---- gradient; each piece of the next row is read as this row's leaves.  ci: 0 without
     // entries, NaN for a bad row
     const bool live = some && !bad;
     const float ci = bad ? quiet_nan() : some ? sc : 0.f;
-    const float kW = ci * W, k1 = REST ? ci * o.k : kW;
+    const float kW = ci * W, k1 = REST ? ci * outside_factor(m, st.s, so.m, so.s, W, rest, a) : kW;
     const float ref = REST ? stat_ref(so.m) : m, shift = REST ? 0.f : -L;
     if (tid < ntail) {
       const float p = __builtin_amdgcn_exp2f(fmaf(xt - ref, a, shift));
@@ -297,8 +312,10 @@ __global__ __launch_bounds__(NT, fused_waves(RES)) void distill_fused_kernel(
     const float q = tid < K ? sq[tid] : 0.f;             // entries of q = 0 add nothing, whatever the student gives them
     float l = q != 0.f ? q * (slq[tid] - ((sx[tid] - m) * inv_temp - LN2 * L)) : 0.f;
     l = block_reduce<NT>(l, 0.f, red[4], OpAdd{}, tid);
-    if (o.use) l += rest * (LN2 * __log2f(rest) - o.lnR);
-    if (tid == 0) loss[r] = bad ? quiet_nan() : some ? l : 0.f;
+    if (tid == 0) {
+      if constexpr (REST) l += rest_loss(m, L, so.m, so.s, rest, inv_temp);
+      loss[r] = bad ? quiet_nan() : some ? l : 0.f;
+    }
   }
 }
 
@@ -385,7 +402,7 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
   bool some;
   if constexpr (REST) {
     if (mine) atomicOr(&bits[(id - vstart) >> 5], 1u << ((id - vstart) & 31));
-    const double qd = te.mass(r, id, z, lq), Q = block_sum<NT>(qd, redq, tid);
+    const double qd = te.mass(r, id, z, lq), Q = block_sum(qd, (te.K + 63) / 64, redq, tid);
     q = (float)qd;
     n = (float)Q;
     some = !(Q == 0.0);
@@ -413,7 +430,7 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
     stat_move<PLAIN>(st, mn, a);
     stat_move<PLAIN>(in, mn, a);
     st.s += in.s;
-    block_stat2<NT>(st, so, a, red3, tid);
+    block_stat2<NT>(st, so, NT / 64, a, red3, tid);
   } else {
     st = block_stat<PLAIN, NT>(st, a, red3[0], tid);
     so = stat_empty();
@@ -425,9 +442,8 @@ __global__ __launch_bounds__(NT, 8) void distill_stats_kernel(const void* __rest
   const float xq = block_reduce<NT>(use ? q * (x - stat_ref(st.m)) : 0.f, 0.f, red[3], OpAdd{}, tid);
   const float ql = block_reduce<NT>(mine ? q : 0.f, 0.f, red[4], OpAdd{}, tid);
   float l = block_reduce<NT>(use ? q * (lq - ((x - st.m) * inv_temp - LN2 * L)) : 0.f, 0.f, red[5], OpAdd{}, tid);
-  const Outside o = REST ? outside(st.m, st.s, so.m, so.s, n + rest, rest, a, inv_temp) : Outside{};
-  if (o.use) l += rest * (LN2 * __log2f(rest) - o.lnR);
   if (tid == 0) {
+    if constexpr (REST) l += rest_loss(st.m, L, so.m, so.s, rest, inv_temp);
     loss[r] = l;
     const float row_stats[ST_COLS] = {st.m, st.s, so.m, so.s, xq, ql, REST ? rest : stat_ref(zm), n, 1.f};
 #pragma unroll
@@ -531,9 +547,8 @@ __global__ __launch_bounds__(GRAD_NT) void distill_grad_kernel(const void* logit
     sqs[tid] = qs;
   }
   lds_barrier();
-  const Outside o = REST ? outside(m, s, st[ST_MO], st[ST_U], W, rest, a, inv_temp) : Outside{};
   const float sc = (rows ? rows[r] : 1.f) * (scale_ptr ? scale_ptr[0] : scale_h) * inv_temp;
-  const float k1 = sc * (REST ? o.k : W), ref = REST ? stat_ref(st[ST_MO]) : m, shift = REST ? 0.f : -L;
+  const float k1 = sc * (REST ? outside_factor(m, s, st[ST_MO], st[ST_U], W, rest, a) : W), ref = REST ? stat_ref(st[ST_MO]) : m, shift = REST ? 0.f : -L;
 #pragma unroll
   for (int j = 0; j < GRAD_UN; ++j) {
     if (c0 + j * GRAD_NT >= nfull) continue;
@@ -550,8 +565,10 @@ __global__ __launch_bounds__(GRAD_NT) void distill_grad_kernel(const void* logit
     store1<DT>(orow, scol[h - 1], sc * fmaf(W, __builtin_amdgcn_exp2f(fmaf(sx[h - 1] - m, a, -L)), -sqs[h - 1]));
   if (all) {
     float l = block_reduce<GRAD_NT>(q != 0.f ? q * (lq + LN2 * L) : 0.f, 0.f, red, OpAdd{}, tid) - inv_temp * st[ST_XQ];
-    if (o.use) l += rest * (LN2 * __log2f(rest) - o.lnR);
-    if (tid == 0) loss[r] = l;
+    if (tid == 0) {
+      if constexpr (REST) l += rest_loss(m, L, st[ST_MO], st[ST_U], rest, inv_temp);
+      loss[r] = l;
+    }
   }
 }
 

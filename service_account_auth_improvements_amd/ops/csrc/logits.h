@@ -195,7 +195,7 @@ __device__ __forceinline__ float block_reduce(float v, float neutral, float* red
   const int l = tid & 15;
   return lane_value(row_reduce(l < NT / 64 ? red[l] : neutral, neutral, op), 15);
 }
-// the same sum in 64 bits
+// a sum in 64 bits, of what the first `waves` waves (four at most) hold; the others skip it
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_add(double v) {
   const u32x2 p = __builtin_bit_cast(u32x2, v);
@@ -204,27 +204,26 @@ __device__ __forceinline__ double dpp_add(double v) {
   for (int i = 0; i < 2; ++i) q[i] = (u32)__builtin_amdgcn_update_dpp(0, (int)p[i], CTRL, ROWS, 0xf, false);
   return v + __builtin_bit_cast(double, q);
 }
-__device__ __forceinline__ double row_sum(double v) {
-  v = dpp_add<0x111, 0xf>(v);
-  v = dpp_add<0x112, 0xf>(v);
-  v = dpp_add<0x114, 0xf>(v);
-  return dpp_add<0x118, 0xf>(v);
-}
 __device__ __forceinline__ double lane_value(double v, int lane) {
   u32x2 p = __builtin_bit_cast(u32x2, v);
 #pragma unroll
   for (int i = 0; i < 2; ++i) p[i] = (u32)__builtin_amdgcn_readlane((int)p[i], lane);
   return __builtin_bit_cast(double, p);
 }
-template <int NT>
-__device__ __forceinline__ double block_sum(double v, double* red, int tid) {
-  v = row_sum(v);
-  v = dpp_add<0x142, 0xa>(v);
-  v = lane_value(dpp_add<0x143, 0xc>(v), 63);
-  if ((tid & 63) == 0) red[tid >> 6] = v;
+__device__ __forceinline__ double block_sum(double v, int waves, double* red, int tid) {
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (wave < waves) {
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    v = lane_value(dpp_add<0x143, 0xc>(v), 63);
+    if ((tid & 63) == 0) red[wave] = v;
+  }
   lds_barrier();
-  const int l = tid & 15;
-  return lane_value(row_sum(l < NT / 64 ? red[l] : 0.0), 15);
+  v = (tid & 3) < waves ? red[tid & 3] : 0.0;
+  return lane_value(dpp_add<0x112, 0xf>(dpp_add<0x111, 0xf>(v)), 3);
 }
 
 // Running softmax of a row part: m = greatest logit, s = sum 2^((x-m) a), and for the entropy (MOMENT)
@@ -275,11 +274,11 @@ __device__ __forceinline__ RowStat block_stat(RowStat r, float a, RowStat* red, 
   return lanes_stat<KIND, 16>(l < NT / 64 ? red[l] : stat_empty(), a);
 }
 
-// two parts at once
+// two parts at once; in waves from `waves` on p is q
 template <int NT>
-__device__ __forceinline__ void block_stat2(RowStat& p, RowStat& q, float a, RowStat (*red)[2], int tid) {
-  p = lanes_stat<PLAIN, 64>(p, a);
+__device__ __forceinline__ void block_stat2(RowStat& p, RowStat& q, int waves, float a, RowStat (*red)[2], int tid) {
   q = lanes_stat<PLAIN, 64>(q, a);
+  p = __builtin_amdgcn_readfirstlane(tid >> 6) < waves ? lanes_stat<PLAIN, 64>(p, a) : q;
   if ((tid & 63) == 0) { red[tid >> 6][0] = p; red[tid >> 6][1] = q; }
   lds_barrier();
   const int l = tid & 15;
