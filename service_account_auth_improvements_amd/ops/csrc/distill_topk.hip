@@ -612,8 +612,8 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
   const float temp = (float)temperature;
   const size_t lds = lse ? ((size_t)V + 31) / 32 * 4 : 0;
   if (lds > BITS_MAX) return 2;
+  if (rows == 0) return 0;
   if (mode == KD_FUSED && fits_registers(dt, V)) {
-    if (rows == 0) return 0;
     const long bytes = (long)V * (dt == DT_FP32 ? 4 : 2);
     const int keep = rows * bytes <= CACHE_BYTES || (((size_t)out | (size_t)(ldo * (dt == DT_FP32 ? 4 : 2))) & (LINE - 1));
     by_type(dt, [&](auto DTc) {
