@@ -19,7 +19,6 @@ the random-init benchmark model can be driven end to end without downloads.
 from __future__ import annotations
 
 import argparse
-import itertools
 import json
 import logging
 import math
@@ -51,6 +50,30 @@ class HFTokenizer:
 
     def decode(self, ids):
         return self.t.decode(ids)
+
+
+OFFSET_WINDOW = 64            # tokens decoded again at most while a character stays unfinished
+
+
+def text_offsets(tok, ids: List[int], text: str) -> List[int]:
+    """Where each token starts in ``text``, the decoded ``ids``: the length of what the tokens before it
+    decode to, as far as that is in the text (the bytes of an unfinished character are not yet).  A
+    tokenizer may decode a token differently at the start, so each step decodes from a token back."""
+    offsets, a, b, base = [], 0, 0, 0     # tokens up to b make text[:base]; tokens from a on are decoded
+    head = ""                             # decoded a to b
+    for j in range(len(ids)):
+        piece = tok.decode(ids[a:j])
+        new = piece[len(head):]
+        pos = base + len(os.path.commonprefix([new, text[base:base + len(new)]]))
+        final = pos == base + len(new)
+        if j - b > OFFSET_WINDOW:
+            pos, final = min(base + len(new), len(text)), True
+        elif new.endswith("\ufffd"):
+            final = False                 # a character's first bytes, or bytes of no character
+        offsets.append(pos)
+        if final and j > b:
+            a, b, base, head = b, j, pos, tok.decode(ids[b:j])
+    return offsets
 
 
 def create_app(sched: Scheduler, model_name: str, tokenizer=None, registry=None):
@@ -186,7 +209,7 @@ def create_app(sched: Scheduler, model_name: str, tokenizer=None, registry=None)
             tops.append(d)
         return {"tokens": texts, "token_logprobs": [num(v) for v in r.token_logprobs],
                 "top_logprobs": tops if r.logprobs else None,
-                "text_offset": list(itertools.accumulate(map(len, texts[:-1]), initial=0)) if texts else []}
+                "text_offset": text_offsets(tok, r.output, tok.decode(r.output))}
 
     @app.post("/v1/completions")
     def completions():

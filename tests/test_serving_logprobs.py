@@ -105,3 +105,57 @@ def test_scheduler_records_on_the_gpu():
     assert not reqs[-1].token_logprobs
     for r in reqs[:-1]:
         _check_against_forward(eng, r, 5e-2)
+
+
+class _Written:
+    """A scheduler that answers every request with given tokens."""
+
+    e = None
+
+    def __init__(self, output):
+        self.output = output
+
+    def submit(self, r):
+        r.output = list(self.output)
+        r.token_logprobs = [-1.0] * len(r.output)
+        r.top_logprobs = [[(t, -1.0)] for t in r.output]
+        r.t_submit = r.t_first = 0.0
+        r.done.set()
+        return r
+
+
+class _SpaceTokenizer:
+    """Words with a space before each but the first of what is decoded, as sentence-piece vocabularies are."""
+
+    def encode(self, text):
+        return [len(w) for w in text.split()]
+
+    def decode(self, ids):
+        return " ".join("w" * i for i in ids)
+
+
+@pytest.mark.parametrize("text", ["é!", "aé漢😀b", "", "plain", "😀😀"])
+def test_text_offsets_lie_in_the_text(text):
+    """A token's offset is where its first character starts; the bytes of one character share theirs."""
+    app = create_app(_Written(text.encode()), "m").test_client()
+    c = app.post("/v1/completions", json={"prompt": "a", "max_tokens": 4, "logprobs": 1}).json["choices"][0]
+    assert c["text"] == text
+    want = [i for i, ch in enumerate(text) for _ in ch.encode()]
+    assert c["logprobs"]["text_offset"] == want
+
+
+def test_text_offsets_of_bytes_that_are_no_text():
+    # two bytes of no character, one, two that start a character which never ends, one, 900 as the first
+    out = [255, 254, 65, 0xE2, 0x82, 66] + [255] * 900 + [67]
+    app = create_app(_Written(out), "m").test_client()
+    c = app.post("/v1/completions", json={"prompt": "a", "max_tokens": 4, "logprobs": 0}).json["choices"][0]
+    assert c["text"] == "��A�B" + "�" * 900 + "C"
+    off = c["logprobs"]["text_offset"]
+    assert off[:4] == [0, 1, 2, 3] and off[4] in (3, 4) and off[5:] == list(range(4, 4 + 902))
+
+
+def test_text_offsets_where_a_first_space_is_dropped():
+    app = create_app(_Written([3, 1, 4, 1, 5]), "m", tokenizer=_SpaceTokenizer()).test_client()
+    c = app.post("/v1/completions", json={"prompt": "a", "max_tokens": 4, "logprobs": 1}).json["choices"][0]
+    off = c["logprobs"]["text_offset"]
+    assert [c["text"][a:b].strip() for a, b in zip(off, off[1:] + [None])] == ["www", "w", "wwww", "w", "wwwww"]
