@@ -325,6 +325,11 @@ at::Tensor check_tokens(const at::Tensor& tok, const at::Tensor& x, const char* 
               op, ": tokens must be int64 [T] on the logits' device");
   return tok.contiguous();
 }
+// return codes of 1000 and more are a launch's error
+void check_launched(int rc, const char* op) {
+  TORCH_CHECK(rc < 1000, op, ": launch failed: ", hipGetErrorString((hipError_t)(rc - 1000)));
+  check_rc(rc, op);
+}
 // where the gradient goes: the logits themselves, or a tensor that does not overlap them
 void check_grad_out(const at::Tensor& x, const at::Tensor& o, const char* op) {
   const int64_t T = x.size(0), V = x.size(1);
@@ -368,11 +373,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log
   const int64_t scratch_bytes = kf_token_logprobs_scratch(dt, T, (int)x.size(1), (int)top);
   at::Tensor scratch;
   if (scratch_bytes > 0) scratch = at::empty({scratch_bytes / 4}, f32);
-  check_rc(kf_token_logprobs(x.data_ptr(), dt, x.stride(0), T, (int)x.size(1), tok.data_ptr<int64_t>(), ignore_index,
-                             (float)temperature, logp.data_ptr<float>(), entropy.data_ptr<float>(),
-                             stats.data_ptr<float>(), (int)top, ids.data_ptr<int64_t>(), tlp.data_ptr<float>(),
-                             scratch_bytes > 0 ? scratch.data_ptr() : nullptr, cur_stream()),
-           op);
+  check_launched(kf_token_logprobs(x.data_ptr(), dt, x.stride(0), T, (int)x.size(1), tok.data_ptr<int64_t>(), ignore_index,
+                                   (float)temperature, logp.data_ptr<float>(), entropy.data_ptr<float>(),
+                                   stats.data_ptr<float>(), (int)top, ids.data_ptr<int64_t>(), tlp.data_ptr<float>(),
+                                   scratch_bytes > 0 ? scratch.data_ptr() : nullptr, cur_stream()),
+                 op);
   return {logp, entropy, stats, ids, tlp};
 }
 
@@ -391,12 +396,12 @@ at::Tensor token_logprobs_bwd(const at::Tensor& x, const at::Tensor& tokens, con
   const auto tok = check_tokens(tokens, x, op);
   const at::Tensor fresh = grad_out(x, out, op);
   const at::Tensor& d = out.has_value() ? *out : fresh;
-  check_rc(kf_token_logprobs_bwd(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), x.size(0), (int)x.size(1),
-                                 tok.data_ptr<int64_t>(), ignore_index, stats.data_ptr<float>(),
-                                 entropy.data_ptr<float>(), dlogp.has_value() ? dlogp->data_ptr<float>() : nullptr,
-                                 dentropy.has_value() ? dentropy->data_ptr<float>() : nullptr, (float)temperature,
-                                 cur_stream()),
-           op);
+  check_launched(kf_token_logprobs_bwd(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), x.size(0), (int)x.size(1),
+                                       tok.data_ptr<int64_t>(), ignore_index, stats.data_ptr<float>(),
+                                       entropy.data_ptr<float>(), dlogp.has_value() ? dlogp->data_ptr<float>() : nullptr,
+                                       dentropy.has_value() ? dentropy->data_ptr<float>() : nullptr, (float)temperature,
+                                       cur_stream()),
+                 op);
   return fresh;
 }
 
@@ -451,14 +456,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> distill_topk(const at::Tensor& x,
   TORCH_CHECK(mode != 1 || !out.has_value(), op, ": out goes with a gradient");
   const at::Tensor fresh = mode == 1 ? at::empty({0, 0}, x.options()) : grad_out(x, out, op);
   const at::Tensor& d = out.has_value() ? *out : fresh;
-  check_rc(kf_distill_topk(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), T, (int)V, vocab_start, vocab_size, ids.data_ptr(),
-                           ids.scalar_type() == at::kInt ? 1 : 0, ids.stride(0), z.data_ptr(), zt, z.stride(0),
-                           lse.has_value() ? lse->data_ptr<float>() : nullptr, (int)K, temperature,
-                           scale.has_value() ? scale->data_ptr<float>() : nullptr, (float)scale_h,
-                           rows.has_value() ? rows->data_ptr<float>() : nullptr,
-                           want_loss ? loss.data_ptr<float>() : nullptr, st, (int)mode,
-                           cur_stream()),
-           op);
+  check_launched(kf_distill_topk(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), T, (int)V, vocab_start, vocab_size, ids.data_ptr(),
+                                 ids.scalar_type() == at::kInt ? 1 : 0, ids.stride(0), z.data_ptr(), zt, z.stride(0),
+                                 lse.has_value() ? lse->data_ptr<float>() : nullptr, (int)K, temperature,
+                                 scale.has_value() ? scale->data_ptr<float>() : nullptr, (float)scale_h,
+                                 rows.has_value() ? rows->data_ptr<float>() : nullptr,
+                                 want_loss ? loss.data_ptr<float>() : nullptr, st, (int)mode,
+                                 cur_stream()),
+                 op);
   return {loss, part, fresh};
 }
 

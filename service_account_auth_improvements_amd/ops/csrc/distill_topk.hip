@@ -613,6 +613,7 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
   const size_t lds = lse ? ((size_t)V + 31) / 32 * 4 : 0;
   if (lds > BITS_MAX) return 2;
   if (rows == 0) return 0;
+  Launcher launch;
   if (mode == KD_FUSED && fits_registers(dt, V)) {
     const long bytes = (long)V * (dt == DT_FP32 ? 4 : 2);
     const int keep = rows * bytes <= CACHE_BYTES || (((size_t)out | (size_t)(ldo * (dt == DT_FP32 ? 4 : 2))) & (LINE - 1));
@@ -620,8 +621,8 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
       auto go = [&](auto NTc, auto Sc, auto Rc) {
         constexpr int DT = decltype(DTc)::value, NT = decltype(NTc)::value, RES = decltype(Sc)::value;
         const unsigned grid = (unsigned)std::min<long>(rows, (long)cu_count() * (256 * fused_waves(RES) / NT));
-        distill_fused_kernel<DT, NT, RES, decltype(Rc)::value><<<grid, NT, 0, s>>>(
-            logits, ld, out, ldo, rows, V, te, temp, scale_ptr, scale_h, loss, keep);
+        launch(distill_fused_kernel<DT, NT, RES, decltype(Rc)::value>, grid, NT, 0, s, logits, ld, out, ldo, rows, V, te,
+               temp, scale_ptr, scale_h, loss, keep);
       };
       auto by_rest = [&](auto NTc, auto Sc) {
         if (lse) go(NTc, Sc, std::true_type{});
@@ -636,7 +637,7 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
       else if (np <= 512 * RES_MAX) by_rest(std::integral_constant<int, 512>{}, Long{});
       else by_rest(std::integral_constant<int, 1024>{}, Long{});
     });
-    return 0;
+    return launch.rc;
   }
   if (mode != KD_GRAD) {
     if (!stats) return 3;
@@ -650,8 +651,8 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
         constexpr int DT = decltype(DTc)::value;
         auto go = [&](auto NTc, auto Rc) {
           constexpr int NT = decltype(NTc)::value;
-          distill_stats_kernel<DT, NT, decltype(Rc)::value><<<n, NT, lds, s>>>(
-              (const char*)logits + r0 * ld * Elem<DT>::bytes, ld, V, vstart, t, temp, loss + r0, stats + r0 * ST_COLS);
+          launch(distill_stats_kernel<DT, NT, decltype(Rc)::value>, n, NT, lds, s,
+                 (const char*)logits + r0 * ld * Elem<DT>::bytes, ld, V, vstart, t, temp, loss + r0, stats + r0 * ST_COLS);
         };
         auto by_rest = [&](auto NTc) {
           if (lse) go(NTc, std::true_type{});
@@ -678,7 +679,7 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
         t.z = (const char*)z + r0 * ldz * (zt == DT_FP32 ? 4 : 2);
         if (lse) t.lse = lse + r0;
         auto go = [&](auto Rc) {
-          distill_grad_kernel<DT, decltype(Rc)::value><<<(unsigned)(n * parts), GRAD_NT, 0, s>>>(
+          launch(distill_grad_kernel<DT, decltype(Rc)::value>, (unsigned)(n * parts), GRAD_NT, 0, s,
               (const char*)logits + r0 * ld * Elem<DT>::bytes, ld, (char*)out + r0 * ldo * Elem<DT>::bytes, ldo, V, parts,
               vstart, t, temp, scale_ptr, scale_h, row_scale ? row_scale + r0 : nullptr,
               // the statistics' launch wrote the loss of an undivided row already
@@ -689,7 +690,7 @@ int kf_distill_topk(const void* logits, int dt, long ld, void* out, long ldo, lo
       }
     });
   }
-  return 0;
+  return launch.rc;
 }
 
 }  // extern "C"

@@ -12,6 +12,7 @@
 // distillation's time): it is exact where it matters (x near m), however great m is, and stays
 // finite for logits at the type's lowest value, where x a would overflow.
 #pragma once
+#include <tuple>
 #include <type_traits>
 
 #include "common.h"
@@ -287,6 +288,21 @@ __device__ __forceinline__ void block_stat2(RowStat& p, RowStat& q, int waves, f
 }
 
 constexpr long ROWS_PER_LAUNCH = 1 << 20;   // a launch holds less than 2^32 threads
+
+// Launches kernels; rc is 0 or, from LAUNCH_RC on, the first launch's error.
+constexpr int LAUNCH_RC = 1000;
+struct Launcher {
+  int rc = 0;
+  template <typename... P, typename... A>
+  void operator()(void (*kernel)(P...), unsigned grid, unsigned block, size_t lds, hipStream_t s, A... a) {
+    std::tuple<P...> args(static_cast<P>(a)...);
+    const hipError_t e = std::apply([&](P&... p) {
+      void* at[] = {(void*)&p...};
+      return hipLaunchKernel((const void*)kernel, dim3(grid), dim3(block), at, lds, s);
+    }, args);
+    if (rc == 0 && e != hipSuccess) rc = LAUNCH_RC + (int)e;
+  }
+};
 
 // f(std::integral_constant<int, DT>) for the type dt
 template <typename F>

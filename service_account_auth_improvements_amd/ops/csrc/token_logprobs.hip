@@ -459,6 +459,7 @@ int kf_token_logprobs(const void* logits, int dt, long ld, long rows, int V, con
   if (V < 1 || k < 0 || k > V || k > TOP_MAX || dt < DT_BF16 || dt > DT_FP32) return 1;
   if (rows == 0) return 0;
   const float a = LOG2E / temp, inv = 1.f / temp;
+  Launcher launch;
   by_type(dt, [&](auto DTc) {
     constexpr int DT = decltype(DTc)::value;
     const int np = (V + Elem<DT>::N - 1) / Elem<DT>::N, parts = split_parts(rows, np, k);
@@ -470,11 +471,13 @@ int kf_token_logprobs(const void* logits, int dt, long ld, long rows, int V, con
       // the parts are of equal size, so the last ones may be empty: as many as hold a piece
       const int used = cdiv(np, per);
       if (k > 0)
-        logprobs_part_kernel<DT, true><<<(unsigned)(rows * used), PART_NT, 0, s>>>(logits, ld, V, a, k, used, per, part, keys);
+        launch(logprobs_part_kernel<DT, true>, (unsigned)(rows * used), PART_NT, 0, s, logits, ld, V, a, k, used, per,
+               part, keys);
       else
-        logprobs_part_kernel<DT, false><<<(unsigned)(rows * used), PART_NT, 0, s>>>(logits, ld, V, a, 0, used, per, part, keys);
-      logprobs_join_kernel<DT><<<(unsigned)rows, k > 0 ? JOIN_NT : 64, 0, s>>>(logits, ld, V, tokens, ignore, a, inv, k,
-                                                                              used, part, keys, o);
+        launch(logprobs_part_kernel<DT, false>, (unsigned)(rows * used), PART_NT, 0, s, logits, ld, V, a, 0, used, per,
+               part, keys);
+      launch(logprobs_join_kernel<DT>, (unsigned)rows, k > 0 ? JOIN_NT : 64, 0, s, logits, ld, V, tokens, ignore, a, inv, k,
+             used, part, keys, o);
       return;
     }
     for (long r0 = 0; r0 < rows; r0 += ROWS_PER_LAUNCH) {
@@ -483,7 +486,8 @@ int kf_token_logprobs(const void* logits, int dt, long ld, long rows, int V, con
       const Result o{logp + r0, entropy + r0, stats + 2 * r0, k > 0 ? top + r0 * k : nullptr, k > 0 ? ids + r0 * k : nullptr};
       auto go = [&](auto NTc, auto TOPc) {
         constexpr int NT = decltype(NTc)::value;
-        logprobs_kernel<DT, NT, decltype(TOPc)::value><<<n, NT, 0, s>>>(x, ld, V, tokens + r0, ignore, a, inv, k, o);
+        launch(logprobs_kernel<DT, NT, decltype(TOPc)::value>, n, NT, 0, s, x, ld, V, tokens + r0, ignore, a, inv, k,
+               o);
       };
       // eight to sixteen pieces a thread: 4000 rows of 128256 bf16 logits take 157 us with 1024
       // threads and 172 with 512, of 32000 logits 52 and 47.  With alternatives smaller blocks: more
@@ -502,7 +506,7 @@ int kf_token_logprobs(const void* logits, int dt, long ld, long rows, int V, con
       }
     }
   });
-  return 0;
+  return launch.rc;
 }
 
 int kf_token_logprobs_bwd(const void* logits, int dt, long ld, void* out, long ldo, long rows, int V, const long* tokens,
@@ -510,19 +514,20 @@ int kf_token_logprobs_bwd(const void* logits, int dt, long ld, void* out, long l
                           float temp, hipStream_t s) {
   if (V < 1 || dt < DT_BF16 || dt > DT_FP32) return 1;
   const float a = LOG2E / temp, inv = 1.f / temp;
+  Launcher launch;
   by_type(dt, [&](auto DTc) {
     constexpr int DT = decltype(DTc)::value;
     const int parts = cdiv((V + Elem<DT>::N - 1) / Elem<DT>::N, BWD_NT * BWD_UN);
     const long per = std::max<long>(1, (1L << 23) / parts);     // rows of a launch: less than 2^32 threads
     for (long r0 = 0; r0 < rows; r0 += per) {
       const long n = std::min(per, rows - r0);
-      logprobs_bwd_kernel<DT><<<(unsigned)(n * parts), BWD_NT, 0, s>>>(
+      launch(logprobs_bwd_kernel<DT>, (unsigned)(n * parts), BWD_NT, 0, s,
           (const char*)logits + r0 * ld * Elem<DT>::bytes, ld, (char*)out + r0 * ldo * Elem<DT>::bytes, ldo, V, parts,
           tokens + r0, ignore, stats + 2 * r0, entropy + r0, dlogp ? dlogp + r0 : nullptr, dent ? dent + r0 : nullptr, a,
           inv);
     }
   });
-  return 0;
+  return launch.rc;
 }
 
 }  // extern "C"

@@ -1,8 +1,13 @@
-"""Calls of the operators over logits at the limits of what they take: no rows."""
+"""Calls of the operators over logits at the limits of what they take: no rows, the longest rows, and a
+launch that fails."""
+import ctypes
+
 import pytest
 import torch
 
+import logits_oracle as oracle
 from service_account_auth_improvements_amd import ops
+from service_account_auth_improvements_amd.ops import _ext
 
 
 def _no_rows(device, V, lse):
@@ -35,3 +40,32 @@ def test_no_rows(V, lse):
 @pytest.mark.parametrize("V", [1, 100, 300001])
 def test_no_rows_gpu(V, lse):
     _no_rows("cuda:0", V, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [491519, 491520])
+def test_longest_rows_with_a_teacher_lse(V, dtype):
+    g = torch.Generator().manual_seed(V)
+    x = (torch.randn(2, V, generator=g) * 2).to(dtype)
+    ids = torch.cat([torch.randint(0, V - 1, (2, 63), generator=g).sort(1).values, torch.full((2, 1), V - 1)], 1)
+    z = torch.randn(2, 64, generator=g) + 4
+    lse = torch.logsumexp(z, 1) + 0.3
+    rl, rd, size, lsize = oracle.distill(x, ids, z, 1.0, lse)
+    loss, d = ops.distill_topk_fused(x.cuda(), ids.cuda(), z.cuda(), 1.0, 1.0, lse.cuda())
+    oracle.close(loss, rl, (1 + lsize) * 4 * oracle.sum_bound(V), "loss")
+    oracle.close(d, rd, oracle.grad_bound(rd, size, 60.0, V, dtype), "dlogits")
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="launches with null pointers, which only fail where there is no device")
+def test_a_launch_that_fails_is_returned():
+    lib = ctypes.CDLL(str(_ext.lib_path()))
+    n, L, I, F, D = ctypes.c_void_p(0), ctypes.c_long, ctypes.c_int, ctypes.c_float, ctypes.c_double
+    assert lib.kf_token_logprobs(n, I(0), L(64), L(1), I(64), n, L(-100), F(1), n, n, n, I(0), n, n, n, n) >= 1000
+    assert lib.kf_token_logprobs_bwd(n, I(0), L(64), n, L(64), L(1), I(64), n, L(-100), n, n, n, n, F(1), n) >= 1000
+    for mode, V in ((0, 64), (0, 4), (1, 64), (2, 64)):
+        stats = (ctypes.c_float * 16)()
+        assert lib.kf_distill_topk(n, I(0), L(V), n, L(V), L(1), I(V), L(0), L(V), n, I(0), L(1), n, I(0), L(1), n, I(1), D(1), n, F(1), n, n,
+                                   stats, I(mode), n) >= 1000
+    # nothing to launch
+    assert lib.kf_token_logprobs(n, I(0), L(64), L(0), I(64), n, L(-100), F(1), n, n, n, I(0), n, n, n, n) == 0
