@@ -303,7 +303,7 @@ def token_logprobs_bwd(logits, tokens, stats, entropy, dlogp=None, dentropy=None
                        ignore_index=-100, out=None):
     """Gradient of :func:`token_logprobs_fwd`'s logp and entropy: dlogits in the logits' type, for
     upstream gradients ``dlogp`` / ``dentropy`` (fp32 [T], None: zero).  ``out``: where to write it;
-    ``out=logits`` overwrites them."""
+    ``out=logits`` overwrites them.  Nothing else that the call reads may lie in ``out``."""
     if out is not None:
         torch.autograd.graph.increment_version(out)
     fn = _k().token_logprobs_bwd if logits.is_cuda else reference.token_logprobs_bwd
@@ -338,7 +338,8 @@ def distill_topk_fused(logits, teacher_ids, teacher_logits, scale, temperature=1
     teacher_logits (with a zero ``teacher_lse`` at temperature 1).
 
     Returns (loss rows fp32 [T], dlogits).  dlogits are ``scale`` (a number or one fp32 on the
-    device) times the rows' gradients; ``out`` says where they go (``out=logits``: in place).
+    device) times the rows' gradients; ``out`` says where they go (``out=logits``: in place; nothing
+    else that the call reads may lie there).
     Neither is multiplied by temperature squared.  A row without entries gives 0; an id at or behind
     the vocabulary's end gives NaN.  The same id may appear twice: its entries add up."""
     return _distill(logits, teacher_ids, teacher_logits, teacher_lse, temperature, scale, None, 0, None, DISTILL_FUSED,

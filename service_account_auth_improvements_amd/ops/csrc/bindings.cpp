@@ -330,22 +330,33 @@ void check_launched(int rc, const char* op) {
   TORCH_CHECK(rc < 1000, op, ": launch failed: ", hipGetErrorString((hipError_t)(rc - 1000)));
   check_rc(rc, op);
 }
+// whether out ([T, V], rows of their own) and `a` ([T, n] with unit inner stride, or contiguous) share no
+// byte: they lie apart, or side by side as columns of one buffer
+bool apart(const at::Tensor& out, const at::Tensor& a) {
+  if (out.numel() == 0 || a.numel() == 0) return true;
+  const int64_t To = out.size(0), wo = out.size(1) * out.element_size(), lo = To > 1 ? out.stride(0) * out.element_size() : wo;
+  const int64_t Ta = a.dim() == 2 ? a.size(0) : 1, wa = a.numel() / Ta * a.element_size();
+  const int64_t la = Ta > 1 ? a.stride(0) * a.element_size() : lo;
+  const char *ob = (const char*)out.data_ptr(), *ab = (const char*)a.data_ptr();
+  if (ab + (Ta - 1) * la + wa <= ob || ob + (To - 1) * lo + wo <= ab) return true;
+  const int64_t d = ((ab - ob) % lo + lo) % lo;
+  return la == lo && d >= wo && d + wa <= lo;
+}
+// nothing else that the call reads may lie in out: blocks are done with their rows at different times
+void check_apart(const std::optional<at::Tensor>& out, const at::Tensor& a, const char* op, const char* name) {
+  if (out.has_value()) TORCH_CHECK(apart(*out, a), op, ": out overlaps the ", name);
+}
+void check_apart(const std::optional<at::Tensor>& out, const std::optional<at::Tensor>& a, const char* op, const char* name) {
+  if (a.has_value()) check_apart(out, *a, op, name);
+}
 // where the gradient goes: the logits themselves, or a tensor that does not overlap them
 void check_grad_out(const at::Tensor& x, const at::Tensor& o, const char* op) {
   const int64_t T = x.size(0), V = x.size(1);
   TORCH_CHECK(o.device() == x.device() && o.scalar_type() == x.scalar_type() && o.sizes() == x.sizes() &&
                   (V == 1 || o.stride(1) == 1) && (T <= 1 || o.stride(0) >= V),
               op, ": out must have the logits' type, shape and device, unit inner stride and rows of their own");
-  if (T == 0) return;
-  const int64_t es = x.element_size(), lx = T > 1 ? x.stride(0) : V, lo = T > 1 ? o.stride(0) : V;
-  const char *xb = (const char*)x.data_ptr(), *ob = (const char*)o.data_ptr();
-  const char *xe = xb + ((T - 1) * lx + V) * es, *oe = ob + ((T - 1) * lo + V) * es;
-  bool ok = xe <= ob || oe <= xb || (xb == ob && lx == lo);
-  if (!ok && lx == lo && (ob - xb) % es == 0) {      // columns of one buffer, side by side
-    const int64_t d = (((ob - xb) / es) % lx + lx) % lx;
-    ok = d >= V && d <= lx - V;
-  }
-  TORCH_CHECK(ok, op, ": out overlaps the logits without being them");
+  const bool same = x.data_ptr() == o.data_ptr() && (T <= 1 || x.stride(0) == o.stride(0));
+  TORCH_CHECK(same || apart(o, x), op, ": out overlaps the logits without being them");
 }
 // a new tensor for the gradient, or an empty one where `out` is given and fit to take it
 at::Tensor grad_out(const at::Tensor& x, const std::optional<at::Tensor>& out, const char* op) {
@@ -395,6 +406,11 @@ at::Tensor token_logprobs_bwd(const at::Tensor& x, const at::Tensor& tokens, con
   c10::hip::HIPGuardMasqueradingAsCUDA g(x.device());
   const auto tok = check_tokens(tokens, x, op);
   const at::Tensor fresh = grad_out(x, out, op);
+  check_apart(out, tok, op, "tokens");
+  check_apart(out, stats, op, "stats");
+  check_apart(out, entropy, op, "entropy");
+  check_apart(out, dlogp, op, "dlogp");
+  check_apart(out, dentropy, op, "dentropy");
   const at::Tensor& d = out.has_value() ? *out : fresh;
   check_launched(kf_token_logprobs_bwd(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), x.size(0), (int)x.size(1),
                                        tok.data_ptr<int64_t>(), ignore_index, stats.data_ptr<float>(),
@@ -455,6 +471,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> distill_topk(const at::Tensor& x,
   }
   TORCH_CHECK(mode != 1 || !out.has_value(), op, ": out goes with a gradient");
   const at::Tensor fresh = mode == 1 ? at::empty({0, 0}, x.options()) : grad_out(x, out, op);
+  check_apart(out, ids, op, "ids");
+  check_apart(out, z, op, "teacher logits");
+  check_apart(out, lse, op, "lse");
+  check_apart(out, scale, op, "scale");
+  check_apart(out, rows, op, "row weights");
+  check_apart(out, stats_in, op, "stats");
   const at::Tensor& d = out.has_value() ? *out : fresh;
   check_launched(kf_distill_topk(x.data_ptr(), dt, x.stride(0), d.data_ptr(), d.stride(0), T, (int)V, vocab_start, vocab_size, ids.data_ptr(),
                                  ids.scalar_type() == at::kInt ? 1 : 0, ids.stride(0), z.data_ptr(), zt, z.stride(0),

@@ -1,5 +1,5 @@
-"""Calls of the operators over logits at the limits of what they take: no rows, the longest rows, and a
-launch that fails."""
+"""Calls of the operators over logits at the limits of what they take: no rows, the longest rows, a
+launch that fails, and outputs over inputs."""
 import ctypes
 
 import pytest
@@ -69,3 +69,39 @@ def test_a_launch_that_fails_is_returned():
                                    stats, I(mode), n) >= 1000
     # nothing to launch
     assert lib.kf_token_logprobs(n, I(0), L(64), L(0), I(64), n, L(-100), F(1), n, n, n, I(0), n, n, n, n) == 0
+
+
+@pytest.mark.gpu
+def test_out_over_another_input_is_refused():
+    T, V, K = 4, 128, 5
+    buf = torch.zeros(T, V + 8, device="cuda")
+    x, beside = buf[:, :V], buf[:, V:V + K]
+    other = torch.zeros(T, V, device="cuda")
+    ids, z = torch.arange(K, device="cuda").repeat(T, 1), torch.randn(T, K, device="cuda")
+    f, st, tok = torch.zeros(T, device="cuda"), torch.zeros(T, 2, device="cuda"), torch.zeros(T, dtype=torch.long, device="cuda")
+    stats = ops.distill_topk_stats(x, ids, z)
+    n = stats.shape[1]
+    flat = other.view(-1)
+    whole = flat.view(torch.int64)
+    refused = {
+        "teacher logits": lambda: ops.distill_topk_fused(x, ids, x[:, :K], 1.0, out=x),
+        "teacher logits,": lambda: ops.distill_topk_fused(x, ids, other[:, 3:3 + K], 1.0, out=other),
+        "ids": lambda: ops.distill_topk_fused(x, whole[:T * K].view(T, K), z, 1.0, out=other),
+        "lse": lambda: ops.distill_topk_fused(x, ids, z, 1.0, 1.0, flat[-T:], out=other),
+        "scale": lambda: ops.distill_topk_fused(x, ids, z, flat[7:8], out=other),
+        "stats": lambda: ops.distill_topk_grad(x, ids, z, flat[:T * n].view(T, n), 1.0, out=other),
+        "tokens": lambda: ops.token_logprobs_bwd(x, whole[:T], st, f, f, out=other),
+        "stats,": lambda: ops.token_logprobs_bwd(x, tok, flat[:2 * T].view(T, 2), f, f, out=other),
+        "entropy": lambda: ops.token_logprobs_bwd(x, tok, st, flat[:T], f, out=other),
+        "dlogp": lambda: ops.token_logprobs_bwd(x, tok, st, f, flat[:T], out=other),
+        "dentropy": lambda: ops.token_logprobs_bwd(x, tok, st, f, f, flat[:T], out=other),
+    }
+    for name, call in refused.items():
+        with pytest.raises(RuntimeError, match="out overlaps the " + name.rstrip(",")):
+            call()
+    # beside the logits in one buffer, and the logits themselves: taken
+    beside.copy_(z)
+    x.normal_(generator=torch.Generator("cuda").manual_seed(0))
+    want = ops.distill_topk_fused(x, ids, z, 1.0)
+    got = ops.distill_topk_fused(x, ids, beside, 1.0, out=x)
+    assert torch.equal(got[0], want[0]) and torch.equal(x, want[1]) and torch.equal(beside, z)
