@@ -334,14 +334,14 @@ def distill_topk_fused(logits, teacher_ids, teacher_logits, scale, temperature=1
     teacher_logits [T, K] of any of the three types.  Without ``teacher_lse``, q is the softmax of the
     entries.  With it (fp32 [T]: the log-sum-exp of the teacher's whole row at ``temperature``),
     q = exp(z / temperature - lse), and the teacher's remaining mass is held against the student's
-    mass outside the ids as one bucket; V is at most 491520 then.  Log-probabilities serve as
-    teacher_logits (with a zero ``teacher_lse`` at temperature 1).
+    mass outside the ids as one bucket (left out where there is nothing but -inf); V is at most 491520
+    then.  Log-probabilities serve as teacher_logits (with a zero ``teacher_lse`` at temperature 1).
 
     Returns (loss rows fp32 [T], dlogits).  dlogits are ``scale`` (a number or one fp32 on the
     device) times the rows' gradients; ``out`` says where they go (``out=logits``: in place; nothing
-    else that the call reads may lie there).
-    Neither is multiplied by temperature squared.  A row without entries gives 0; an id at or behind
-    the vocabulary's end gives NaN.  The same id may appear twice: its entries add up."""
+    else that the call reads may lie there).  Neither is multiplied by temperature squared.  A row
+    without entries gives 0; an id at or behind the vocabulary's end gives NaN.  The same id may appear
+    twice: its entries add up."""
     return _distill(logits, teacher_ids, teacher_logits, teacher_lse, temperature, scale, None, 0, None, DISTILL_FUSED,
                     None, out)
 

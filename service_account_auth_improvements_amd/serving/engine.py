@@ -432,7 +432,7 @@ MAX_LOGPROBS = 20             # alternatives a request may ask for
 
 def record_logprobs(logits: torch.Tensor, tokens: List[int], reqs: List["Request"]):
     """Append the log-probability of each request's new token, and its alternatives, for the requests
-    that asked: one ops.token_logprobs_fwd over the batch (the other rows are passed over)."""
+    that asked: one ops.token_logprobs_fwd over the batch (the other rows count as padding)."""
     if all(r.logprobs is None for r in reqs):
         return
     top = min(max(r.logprobs or 0 for r in reqs), logits.shape[1])
